@@ -43,7 +43,8 @@ enum {
   KVD_ERR_NUMERIC = 6    /* device reported a numerical failure */
 };
 
-enum { KVD_DTYPE_F32 = 0, KVD_DTYPE_BF16 = 1 };
+enum { KVD_DTYPE_F32 = 0, KVD_DTYPE_BF16 = 1, KVD_DTYPE_F16 = 2 }; /* F16: the paged calls only */
+enum { KVD_STORE_E4M3 = 0, KVD_STORE_INT8 = 1 };                   /* 8-bit codes of a paged pool */
 enum { KVD_RETENTION_FIFO = 0, KVD_RETENTION_LOWRANK_SURPRISE = 1 };
 
 /* Configuration of one cache group (bug_cache.py:313-540 constructor knobs). */
@@ -271,6 +272,87 @@ size_t kvd_blocked_project_workspace_bytes(int32_t n, int32_t t, int32_t rank_ca
 
 /* Workspace bytes kvd_factored_decode needs for `count` problems. */
 size_t kvd_decode_workspace_bytes(const kvd_config* cfg, int32_t count, int32_t num_q_heads);
+
+/* ------------------------------------------------- 8-bit paged KV cache
+ *
+ * A cache that holds every token, for requests of their own lengths (no
+ * counterpart in the reference; the baseline beside its compressed cache):
+ * keys and values as 8-bit codes in pages of page_size tokens, with one fp32
+ * scale for each (page, KV head): x = code * scale.  Calls on one pool or one
+ * set of tables are ordered by their stream; lengths, tables and slots stay on
+ * the device, and what they hold is checked there: bad slots and page ids are
+ * skipped and set status bits (kvd_paged_check_status). */
+
+typedef struct kvd_paged_pool {
+  void* k; void* v;                 /* codes [num_pages][num_heads][page_size][head_dim] */
+  float* k_scale; float* v_scale;   /* [num_pages][num_heads] */
+  int64_t page_stride, head_stride, slot_stride; /* of the codes, bytes, multiples of 16 */
+  int64_t scale_stride;             /* scales of one page to the next page's, elements */
+  int32_t num_pages, page_size;     /* page_size 16, 32, 64 or 128; num_pages * page_size < 2^31 */
+  int32_t num_heads, head_dim;      /* head_dim 32, 64, 128 or 256 */
+  int32_t store;                    /* KVD_STORE_* */
+  int32_t* status;                  /* [4] device status words, or NULL */
+} kvd_paged_pool;
+
+/* Page tables, slot map and positions of one step.  Request b holds
+ * cached_lens[b] tokens in the first pages of table[b] and gets new_lens[b]
+ * more; new pages come from the top of the free stack free_pages
+ * [0, *free_count) (num_free: its size), in request order.  Writes the new
+ * table entries, lens[b] = cached + new (may be cached_lens), *free_left (may
+ * be free_count), cu_new [batch + 1] (exclusive prefix sums of new_lens), and
+ * per row of the step its slot (page * page_size + offset) and its position;
+ * rows [cu_new[batch], capacity) get slot -1 and position 0.  When pages, table
+ * columns or rows do not suffice, or a length is negative, nothing is
+ * allocated: every slot is -1, cu_new 0, lens = cached_lens, and the status
+ * bit is set.  batch <= 12288. */
+int kvd_page_tables(int32_t batch, int32_t max_pages, int32_t page_size, const int32_t* cached_lens,
+                    const int32_t* new_lens, int32_t* table, int64_t table_stride,
+                    const int32_t* free_pages, int32_t num_free, const int32_t* free_count, int32_t capacity,
+                    int32_t* lens, int32_t* free_left, int32_t* cu_new, int32_t* slots, int32_t* positions,
+                    int32_t* status, kvd_stream_t stream);
+/* Requests with done[b] != 0 give their pages back on top of the free stack,
+ * in request order, and have lens[b] = 0 afterwards. */
+int kvd_page_release(int32_t batch, int32_t max_pages, int32_t page_size, const uint8_t* done, int32_t* lens,
+                     const int32_t* table, int64_t table_stride, int32_t* free_pages, int32_t num_free,
+                     int32_t* free_count, int32_t* status, kvd_stream_t stream);
+
+/* Store keys and values (batch, H, tokens, D): row b * tokens + t goes to
+ * slots[b * tokens + t]; a negative slot is skipped.  Rows that go to one page
+ * must follow one another with ascending slots (as kvd_page_tables gives
+ * them), and a page's slots fill from its first one on.  A page's scale is the
+ * least power of two that fits its largest value; it grows with later calls,
+ * and the codes before them are then rounded again. */
+int kvd_paged_append(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,
+                     kvd_hf_view k, kvd_hf_view v, kvd_stream_t stream);
+
+/* Dense keys and values of the first out_k.tokens tokens of each request, in
+ * the model dtype (the return value a model's own attention reads); rows from
+ * lens[b] on are zero.  batch <= 32767. */
+int kvd_paged_peek(const kvd_paged_pool* pool, int32_t batch, const int32_t* table, int64_t table_stride,
+                   int32_t max_pages, const int32_t* lens, int32_t dtype, kvd_hf_view out_k,
+                   kvd_hf_view out_v, kvd_stream_t stream);
+
+/* Attention over the pages.  Request b's queries are its last tokens: query i
+ * of its n sees tokens t <= lens[b] - n + i, t >= starts[b] (left padding;
+ * starts may be NULL) and, with window > 0, t > lens[b] - n + i - window.  A
+ * row that sees nothing gives zeros and lse -inf.  cu_q [batch + 1] (packed
+ * queries, q_tokens rows in all, max_q the most of one request or 0 for not
+ * known) or NULL (every request has q_tokens).  q: element strides of batch,
+ * head and token, multiples of 16 bytes, unit stride over D.  out
+ * (rows, num_q_heads, D) contiguous, lse (rows, num_q_heads) or NULL: natural
+ * log of the softmax sum.  Rows behind cu_q[batch] are left as they were, or
+ * zero (lse -inf) with fill_tail. */
+int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, const int32_t* table, int64_t table_stride,
+                        int32_t max_pages, const int32_t* lens, const int32_t* starts, const int32_t* cu_q,
+                        int32_t dtype, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                        int32_t q_tokens, int32_t max_q, int32_t num_q_heads, float scaling, int32_t window,
+                        void* out, float* lse, int32_t fill_tail, void* workspace, size_t ws_bytes,
+                        kvd_stream_t stream);
+size_t kvd_paged_attention_workspace_bytes(const kvd_paged_pool* pool, int32_t dtype, int32_t num_q_heads);
+
+/* Read and clear the status words of a pool or of page tables (synchronises
+ * the stream). */
+int kvd_paged_check_status(int32_t* status, kvd_stream_t stream);
 
 /* ------------------------------------------------------------ RoPE angles */
 

@@ -9,6 +9,9 @@ Public surface (drop-in for kvdlra's):
 * :mod:`kvdlra_b200.accounting` -- the float-equivalent charge (accounting.py);
 * :func:`enable_factored_decode` -- a model's decode attention answered by the
   factored kernel over the compressed cache;
+* :mod:`kvdlra_b200.paged` -- an 8-bit paged cache that holds every token, for
+  ragged batches: page tables, the quantising writer, the dense reader and
+  attention over the pages;
 * :mod:`kvdlra_b200.harness` -- chunked prefill and greedy decode drivers.
 
 The compute runs in ``_lib/libkvdlra_b200.so`` (built by
@@ -17,6 +20,7 @@ The compute runs in ``_lib/libkvdlra_b200.so`` (built by
 
 from .cache import BugStreamingCache, BugStreamingLayer, RopeAngles
 from .integrator import augmented_bug_step, blocked_bug_project, blocked_bug_subspace
+from .paged import PagedPool, PageTables, build_page_tables, paged_append, paged_attention, paged_peek
 from .press import BUGPress
 from .attention import enable_factored_decode
 
@@ -24,5 +28,6 @@ __all__ = [
     "BugStreamingCache", "BugStreamingLayer", "RopeAngles",
     "augmented_bug_step", "blocked_bug_project", "blocked_bug_subspace", "BUGPress",
     "enable_factored_decode",
+    "PagedPool", "PageTables", "build_page_tables", "paged_append", "paged_attention", "paged_peek",
 ]
 __version__ = "0.1.0"

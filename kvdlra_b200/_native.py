@@ -93,6 +93,14 @@ def hf_view(t: torch.Tensor | None) -> HFView:
     return HFView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
 
 
+class PagedPool(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("scale_stride", C.c_int64), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+                ("num_heads", C.c_int32), ("head_dim", C.c_int32), ("store", C.c_int32),
+                ("status", C.c_void_p)]
+
+
 _lib: C.CDLL | None = None
 
 
@@ -149,11 +157,21 @@ def lib() -> C.CDLL:
     L.kvd_blocked_project.argtypes = [i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, sz, vp]
     L.kvd_blocked_project_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.kvd_blocked_project_workspace_bytes.restype = sz
+    L.kvd_page_tables.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+    L.kvd_page_release.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, vp, vp]
+    L.kvd_paged_append.argtypes = [P(PagedPool), vp, i32, i32, HFView, HFView, vp]
+    L.kvd_paged_peek.argtypes = [P(PagedPool), i32, vp, i64, i32, vp, i32, HFView, HFView, vp]
+    L.kvd_paged_attention.argtypes = [P(PagedPool), i32, vp, i64, i32, vp, vp, vp, i32, vp, i64, i64, i64, i32, i32,
+                                      i32, f32, i32, vp, vp, i32, vp, sz, vp]
+    L.kvd_paged_attention_workspace_bytes.argtypes = [P(PagedPool), i32, i32]
+    L.kvd_paged_attention_workspace_bytes.restype = sz
+    L.kvd_paged_check_status.argtypes = [vp, vp]
     for name in ("kvd_check_status", "kvd_prefill", "kvd_append", "kvd_consolidate", "kvd_absorb_block", "kvd_peek",
                  "kvd_factored_decode", "kvd_factored_chunk_attention", "kvd_factored_decode_heads",
                  "kvd_factored_chunk_attention_heads", "kvd_bug_step", "kvd_surprise",
                  "kvd_select_topk",
-                 "kvd_profile", "kvd_profile_read", "kvd_blocked_project", "kvd_rope_table"):
+                 "kvd_page_tables", "kvd_page_release", "kvd_paged_append", "kvd_paged_peek", "kvd_paged_attention",
+                 "kvd_paged_check_status", "kvd_profile", "kvd_profile_read", "kvd_blocked_project", "kvd_rope_table"):
         getattr(L, name).restype = C.c_int
     _lib = L
     return L
