@@ -195,6 +195,75 @@ KVD_DEVICE WorkAt find_work(const PagedReqs& a, int cta, int nctas) {
   return r;
 }
 
+// One CTA's pieces of units, in order: `next` moves to the next one.  Every
+// thread that walks them sees the same.
+template <int RT, int TT>
+struct Pieces {
+  const PagedReqs& rq;
+  long left, off_next;
+  int b_next, h_next, rt_next, nrt;
+  bool inside;                    // the next piece is of the same request
+  // the current piece: tiles [tile, tile + n) of unit (b, h, rt), whose own are
+  // [lo / TT, lo / TT + span); `off` of them lie before the piece
+  int b, h, rt, q_len, len, start, rows, lo, hi, span, off, tile, n;
+  KVD_DEVICE Pieces(const PagedReqs& r, const WorkAt& at, int cta) : rq(r) {
+    left = min(at.chunk, at.total - (long)cta * at.chunk);
+    b_next = at.b;
+    off_next = at.off;
+    inside = false;
+  }
+  KVD_DEVICE bool next() {
+    if (left <= 0) return false;
+    if (!inside) {
+      while (true) {
+        if (b_next >= rq.batch) return false;
+        q_len = rq.q_len(b_next);
+        if (q_len > 0 && rq.mine(q_len)) break;
+        ++b_next;
+      }
+      len = rq.len(b_next);
+      start = rq.start(b_next);
+      rows = q_len * rq.G;
+      nrt = (rows + RT - 1) / RT;
+      h_next = rt_next = 0;
+      if (off_next > 0) {
+        long per_head = 0;
+        int l, u;
+        for (int r = 0; r < nrt; ++r) per_head += row_tile_span<RT, TT>(rq, len, q_len, start, r, &l, &u);
+        h_next = (int)(off_next / per_head);
+        off_next -= h_next * per_head;
+        int s;
+        while (off_next >= (s = row_tile_span<RT, TT>(rq, len, q_len, start, rt_next, &l, &u))) { off_next -= s; ++rt_next; }
+      }
+      inside = true;
+    }
+    b = b_next; h = h_next; rt = rt_next;
+    span = row_tile_span<RT, TT>(rq, len, q_len, start, rt, &lo, &hi);
+    off = (int)off_next;
+    tile = lo / TT + off;
+    n = (int)min((long)span - off, left);
+    left -= n;
+    off_next = 0;
+    if (++rt_next == nrt) {
+      rt_next = 0;
+      if (++h_next == rq.H) {
+        inside = false;
+        ++b_next;
+      }
+    }
+    return true;
+  }
+  KVD_DEVICE bool whole() const { return off == 0 && n == span; }
+  // pieces of the unit when the current one begins it and does not finish it
+  KVD_DEVICE int pieces(long chunk) const { return off == 0 && n < span ? 1 + (int)((span - n + chunk - 1) / chunk) : 0; }
+  KVD_DEVICE long out_row(int R) const { return (rq.cu_q ? rq.q0(b) : (long)b * rq.q_tokens) + R / rq.G; }
+  // the tokens that row R sees
+  KVD_DEVICE int row_hi(int R) const { return min(len, len - q_len + R / rq.G + 1); }
+  KVD_DEVICE int row_lo(int R) const {
+    return rq.window > 0 ? max(start, len - q_len + R / rq.G - rq.window + 1) : start;
+  }
+};
+
 // Partial results of a unit that several CTAs share: CTA c's record 0 is the
 // piece of the unit that it continues, record 1 the piece of the unit that it
 // begins and does not finish.  head[c] says what c begins.
@@ -203,22 +272,108 @@ struct PagedPart {
   int4* head;          // [ctas]: request, KV head, row tile, pieces (0: none)
 };
 
+KVD_DEVICE float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+KVD_DEVICE uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+KVD_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+
 struct PagedOut {
   void* out;           // (tokens, Hq, D)
   float* lse;          // (tokens, Hq) or null
   int Hq;
 };
 
+// Joins a split unit's records: M = max m_i, out = sum 2^(m_i - M) O_i / sum
+// 2^(m_i - M) l_i.  One CTA per (CTA of the kernel above, slice of the rows);
+// most have nothing to do.  Bound by the latency of reading the records.
+template <int D, int RT, typename T>
+__global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPart part, PagedOut out, int fill_tail) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (fill_tail && rq.cu_q) {  // rows behind the last request: zeros
+    const long from = (long)max(0, min(rq.cu_q[rq.batch], rq.q_tokens)) * out.Hq, to = (long)rq.q_tokens * out.Hq;
+    const long stride = (long)gridDim.x * gridDim.y * 128;
+    const long at = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + threadIdx.x;
+    for (long e = from * D + at; e < to * D; e += stride) store_f(reinterpret_cast<T*>(out.out) + e, 0.f);
+    if (out.lse)
+      for (long e = from + at; e < to; e += stride) out.lse[e] = -INFINITY;
+  }
+  const int4 u = part.head[blockIdx.x];
+  if (u.w == 0) return;
+  const int b = u.x, h = u.y, rt = u.z, n = u.w;
+  const int rows = min(RT, rq.q_len(b) * rq.G - rt * RT);
+  const long step = 2L * RT * (D + 2);
+  const float* r0 = part.rec + (long)blockIdx.x * step + (long)RT * (D + 2);  // record 1 of the first CTA
+  const float* r1 = part.rec + (long)(blockIdx.x + 1) * step;                 // record 0 of those after it
+  for (int e = blockIdx.y * 128 + threadIdx.x; e < rows * D; e += gridDim.y * 128) {
+    const int r = e / D, d = e % D;
+    float M = r0[RT * D + r];
+#pragma unroll 8
+    for (int i = 0; i < n - 1; ++i) M = fmaxf(M, r1[i * step + RT * D + r]);
+    const float f = M == -INFINITY ? 1.f : exp2_fast(r0[RT * D + r] - M);
+    float L = f * r0[RT * D + RT + r], o = f * r0[r * D + d];
+#pragma unroll 8
+    for (int i = 0; i < n - 1; ++i) {
+      const float* p = r1 + i * step;
+      const float w = M == -INFINITY ? 1.f : exp2_fast(p[RT * D + r] - M);
+      L = fmaf(w, p[RT * D + RT + r], L);
+      o = fmaf(w, p[r * D + d], o);
+    }
+    const int R = rt * RT + r;
+    const long row = (rq.cu_q ? rq.q0(b) : (long)b * rq.q_tokens) + R / rq.G;
+    const int hq = h * rq.G + R % rq.G;
+    store_f(reinterpret_cast<T*>(out.out) + (row * out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
+    if (d == 0 && out.lse) out.lse[row * out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+  }
+}
+
 }  // namespace kvd
 
 namespace kvd_host {
+using kvd::PagedOut; using kvd::PagedPart; using kvd::PagedReqs;
 // Checks of a pool's description; fills the kernels' view of it.
 int paged_pool_view(const kvd_paged_pool* p, kvd::PagedPool* out);
 int paged_sm_count();
-// Attention over the pages on tcgen05 for requests of many rows; the workspace
-// it needs, 0 where it has no kernel for the shape.
-size_t paged_chunk_ws_bytes(const kvd_paged_pool& p, int dtype, int G);
-int launch_paged_chunk(const kvd_paged_pool& p, const kvd::PagedPool& pool, const kvd::PagedReqs& reqs, const int* table,
-                       long table_stride, int dtype, const void* q, long q_sb, long q_sh, long q_st,
-                       float scaling, const kvd::PagedOut& out, void* ws, cudaStream_t s);
+// Attention over the pages on tcgen05, for requests of many rows: whether it
+// takes the shape, its workspace, its launch.
+bool paged_chunk_takes(int head_dim, int dtype);
+size_t paged_chunk_ws_bytes(int head_dim);
+int launch_paged_chunk(const kvd::PagedPool& pool, int D, int store, const PagedReqs& reqs, const int* table, long table_stride,
+                       int dtype, const void* q, long q_sb, long q_sh, long q_st, float scaling_log2, const PagedOut& out,
+                       int fill_tail, void* ws, cudaStream_t s);
+
+inline size_t part_bytes(int ctas, int rt, int D) {
+  return (size_t)ctas * sizeof(int4) + (size_t)ctas * 2 * rt * (D + 2) * sizeof(float);
+}
+inline PagedPart part_at(void* ws, int ctas) {
+  PagedPart p;
+  p.head = (int4*)ws;
+  p.rec = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
+  return p;
+}
+
+template <int D, int RT, typename T>
+int launch_merge(const PagedReqs& rq, const PagedPart& part, const PagedOut& out, int fill_tail, int ctas,
+                        cudaStream_t s) {
+  // starts while the kernel before it drains, and waits for it in the kernel
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, (RT * D + 511) / 512);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  KTimerScope kts_("paged_merge_kernel", s);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kvd::paged_merge_kernel<D, RT, T>, rq, part, out, fill_tail);
+  if (e != cudaSuccess) { set_error("paged_merge_kernel: %s", cudaGetErrorString(e)); return KVD_ERR_CUDA; }
+  return KVD_OK;
+}
+
 }  // namespace kvd_host

@@ -23,8 +23,13 @@
 // Codes are exact in f16.  Q rows are scaled by a power of two to below 2 and
 // rounded to f16 (exact for bf16 and f16 but for elements 2^-13 of the row's
 // largest); an fp32 call splits Q and P into two f16 parts, about 22 bits.
-// P is multiplied by vs / (the largest vs so far) before its rounding to f16,
-// at most 2^-11 relative to the row's largest weight; m, l and O are fp32.
+// P is rounded to f16 (2^-11); m, l and O are fp32.
+//
+// Two references per row, in base 2: m for the sum l of the weights, and mv
+// for O, whose weights carry the page's value scale: p vs = 2^(x - m) (vs
+// 2^(m - mv)), so P's rounding is relative to the largest p vs.  They follow
+// the running maxima only when these pass them by 8 (P <= 2^8): a tile costs
+// one vote instead of reductions over the lanes.
 //
 // Work: (request, KV head, row tile, 128-token tile) is one list, every CTA
 // takes an equal run of it; a unit that spans CTAs leaves records that
@@ -63,17 +68,6 @@ KVD_DEVICE uint32_t transpose_f16x2(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-KVD_DEVICE float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-KVD_DEVICE uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-KVD_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
-
 // CTAs of the few-row kernel per SM: as many as its accumulators and the codes
 // in flight leave registers for without spills
 __host__ __device__ constexpr int rows_per_sm(int D, int nt, bool fp32) {
@@ -114,8 +108,8 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
   constexpr bool SPLIT = sizeof(T) == 4;
   extern __shared__ __align__(16) float osm[];  // [4 warps][RT][D]
   __shared__ int seg_id[kSegPages];
-  __shared__ float seg_ks[kSegPages], seg_w[kSegPages];
-  __shared__ float red[4], sm_m[4][RT], sm_l[4][RT];
+  __shared__ float seg_ks[kSegPages], seg_vs[kSegPages], seg_lv[kSegPages];
+  __shared__ float sm_m[4][RT], sm_l[4][RT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
   const PagedPool& pool = a.pool;
   const PagedReqs& rq = a.reqs;
@@ -123,447 +117,370 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge waits for this grid's end itself
   const WorkAt at = find_work<RT, TT, kRowThreads>(rq, blockIdx.x, gridDim.x);
-  long left = min(at.chunk, at.total - (long)blockIdx.x * at.chunk);
+  Pieces<RT, TT> pc(rq, at, blockIdx.x);
   int4 begun = make_int4(0, 0, 0, 0);
-  int b = at.b;
-  long off = at.off;
 
-  while (left > 0 && b < rq.batch) {
-    // ---- the request, and the unit (head h, row tile rt) that holds its tile `off`
-    const int q_len = rq.q_len(b);
-    if (q_len == 0 || !rq.mine(q_len)) { ++b; continue; }
-    const int len = rq.len(b), start = rq.start(b), rows = q_len * rq.G;
-    const int nrt = (rows + RT - 1) / RT;
-    long per_head = 0;
-    int lo, hi;
-    for (int rt = 0; rt < nrt; ++rt) per_head += row_tile_span<RT, TT>(rq, len, q_len, start, rt, &lo, &hi);
-    int h = (int)(off / per_head), rt = 0;
-    off -= h * per_head;
-    int span;
-    while (off >= (span = row_tile_span<RT, TT>(rq, len, q_len, start, rt, &lo, &hi))) { off -= span; ++rt; }
-    for (; h < rq.H && left > 0; ++h, rt = 0) {
-      for (; rt < nrt && left > 0; ++rt, off = 0) {
-        span = row_tile_span<RT, TT>(rq, len, q_len, start, rt, &lo, &hi);
-        const int n_here = (int)min((long)span - off, left);
-        const int t_begin = (lo / TT + (int)off) * TT, t_end = min(hi, t_begin + n_here * TT);
-        // every row sees [lo_all, hi_all)
-        const int row0 = rt * RT;
-        const int i0 = row0 / rq.G, i1 = min(rows - 1, row0 + RT - 1) / rq.G;
-        const int hi_all = len - q_len + i0 + 1;
-        const int lo_all = rq.window > 0 ? max(start, len - q_len + i1 - rq.window + 1) : start;
+  while (pc.next()) {
+    const int b = pc.b, h = pc.h, row0 = pc.rt * RT, rows = pc.rows, lo = pc.lo, hi = pc.hi;
+    const int t_begin = pc.tile * TT, t_end = min(hi, t_begin + pc.n * TT);
+    // every row sees [lo_all, hi_all)
+    const int hi_all = pc.row_hi(row0), lo_all = pc.row_lo(min(rows - 1, row0 + RT - 1));
 
-        // ---- Q fragments (B operand: k = dims, n = rows), scaled by a power of two per row
-        uint32_t qf[NT][KW][2], ql[SPLIT ? NT : 1][SPLIT ? KW : 1][2];
-        float cq[NT][2];   // this lane's score columns: rows 8 nt + 2j + {0, 1}
-        int lim_lo[NT][2], lim_hi[NT][2];
+    // ---- Q fragments (B operand: k = dims, n = rows), scaled by a power of two per row
+    uint32_t qf[NT][KW][2], ql[SPLIT ? NT : 1][SPLIT ? KW : 1][2];
+    float cq[NT][2];   // this lane's score columns: rows 8 nt + 2j + {0, 1}
+    int lim_lo[NT][2], lim_hi[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int R = row0 + 8 * nt + g;
-          const bool live = R < rows;
-          const int qi = live ? R / rq.G : 0;
-          const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)b * a.q_sb) +
-                         (long)(h * rq.G + (live ? R % rq.G : 0)) * a.q_sh + (long)(rq.q0(b) + qi) * a.q_st;
-          float x[KW][4];
-          float amax = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int R = row0 + 8 * nt + g;
+      const bool live = R < rows;
+      const int qi = live ? R / rq.G : 0;
+      const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)b * a.q_sb) +
+                     (long)(h * rq.G + (live ? R % rq.G : 0)) * a.q_sh + (long)(rq.q0(b) + qi) * a.q_st;
+      float x[KW][4];
+      float amax = 0.f;
 #pragma unroll
-          for (int kk = 0; kk < KW; ++kk) {
-            const int d = D == 32 ? 8 * j + 4 * kk : 64 * (kk >> 2) + 16 * j + 4 * (kk & 3);
-            if constexpr (sizeof(T) == 4) {
-              const float4 f = live ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-              x[kk][0] = f.x; x[kk][1] = f.y; x[kk][2] = f.z; x[kk][3] = f.w;
-            } else {
-              const uint2 u = live ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0u, 0u);
-              const T* e = reinterpret_cast<const T*>(&u);
+      for (int kk = 0; kk < KW; ++kk) {
+        const int d = D == 32 ? 8 * j + 4 * kk : 64 * (kk >> 2) + 16 * j + 4 * (kk & 3);
+        if constexpr (sizeof(T) == 4) {
+          const float4 f = live ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[kk][0] = f.x; x[kk][1] = f.y; x[kk][2] = f.z; x[kk][3] = f.w;
+        } else {
+          const uint2 u = live ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0u, 0u);
+          const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[kk][i] = load_f(e + i);
-            }
+          for (int i = 0; i < 4; ++i) x[kk][i] = load_f(e + i);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[kk][i]));
-          }
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          int e = (int)(__float_as_uint(amax) >> 23) - 127;
-          e = e > 127 ? 0 : max(-100, min(100, e));  // an infinite row keeps its values
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[kk][i]));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      int e = (int)(__float_as_uint(amax) >> 23) - 127;
+      e = e > 127 ? 0 : max(-100, min(100, e));  // an infinite row keeps its values
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-          for (int kk = 0; kk < KW; ++kk) {
+      for (int kk = 0; kk < KW; ++kk) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              const float u = x[kk][2 * p] * down, w = x[kk][2 * p + 1] * down;
-              qf[nt][kk][p] = pack_f16(u, w);
-              if constexpr (SPLIT) {
-                const float2 r = unpack_f16(qf[nt][kk][p]);
-                ql[nt][kk][p] = pack_f16(u - r.x, w - r.y);
-              }
-            }
-          }
-          const float up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scaling;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            cq[nt][c] = __shfl_sync(0xffffffffu, up, (2 * j + c) * 4);
-            const int Rc = min(rows - 1, row0 + 8 * nt + 2 * j + c), ic = Rc / rq.G;
-            lim_hi[nt][c] = min(len, len - q_len + ic + 1);
-            lim_lo[nt][c] = rq.window > 0 ? max(start, len - q_len + ic - rq.window + 1) : start;
+        for (int p = 0; p < 2; ++p) {
+          const float u = x[kk][2 * p] * down, w = x[kk][2 * p + 1] * down;
+          qf[nt][kk][p] = pack_f16(u, w);
+          if constexpr (SPLIT) {
+            const float2 r = unpack_f16(qf[nt][kk][p]);
+            ql[nt][kk][p] = pack_f16(u - r.x, w - r.y);
           }
         }
-
-        float acc[D / 16][NT][4];
-        float m[NT][2], l[NT][2];
+      }
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scaling;
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt)
+      for (int c = 0; c < 2; ++c) {
+        cq[nt][c] = __shfl_sync(0xffffffffu, up, (2 * j + c) * 4);
+        const int Rc = min(rows - 1, row0 + 8 * nt + 2 * j + c);
+        lim_hi[nt][c] = pc.row_hi(Rc);
+        lim_lo[nt][c] = pc.row_lo(Rc);
+      }
+    }
+
+    float acc[D / 16][NT][4];
+    float m[NT][2], mv[NT][2], l[NT][2];  // references of l and of O, see the top
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][nt][i] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = mv[nt][0] = mv[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+
+    const int pg_end = (t_end + page_mask) >> lg;  // pages of the piece
+    for (int pg0 = t_begin >> lg; pg0 < pg_end; ) {
+      // ---- page ids and scales of the next pages (whole tiles)
+      const int t_seg0 = max(t_begin, pg0 << lg);
+      int t_seg1 = t_seg0 + (((pg0 + kSegPages) << lg) - t_seg0) / TT * TT;
+      t_seg1 = min(t_seg1, t_end);
+      const int np = ((t_seg1 + page_mask) >> lg) - pg0;
+      __syncthreads();  // the previous segment's (or unit's) readers are done
+      for (int i = tid; i < np; i += kRowThreads) {
+        int id = a.table[(long)b * a.table_stride + pg0 + i];
+        if (id < 0 || id >= pool.num_pages) {
+          pool.flag(kStatusBounds, kPagedBadPage);
+          id = -1;
+        }
+        const float vs = id < 0 ? 0.f : pool.vs[(long)id * pool.scale_stride + h];
+        seg_id[i] = id;
+        seg_ks[i] = id < 0 ? 0.f : pool.ks[(long)id * pool.scale_stride + h];
+        seg_vs[i] = vs;
+        seg_lv[i] = log2f(vs);
+      }
+      __syncthreads();
+
+      // ---- this warp's tiles
+      const int w_off = warp * WT;
+      auto key_words = [&](int t, uint32_t (&kw)[ST][2][KW]) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
+          const int id = pi < np ? seg_id[pi] : -1;
+          const unsigned char* p = pool.k + (long)id * pool.page_stride + (long)h * pool.head_stride +
+                                   (long)((tb & page_mask) + g) * pool.slot_stride + (D == 32 ? 8 : 16) * j;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (id >= 0) {
+              constexpr int W = KW < 4 ? KW : 4;
+#pragma unroll
+              for (int c = 0; c < KW / W; ++c) load_words<W>(p + 8L * r * pool.slot_stride + 64 * c, &kw[s][r][W * c]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < KW; ++c) kw[s][r][c] = 0u;
+            }
+          }
+        }
+      };
+      auto value_words = [&](int t, uint32_t (&vw)[ST][4][VW]) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+          const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
+          const int id = pi < np ? seg_id[pi] : -1;
+          const unsigned char* p = pool.v + (long)id * pool.page_stride + (long)h * pool.head_stride +
+                                   (long)((tb & page_mask) + 2 * j) * pool.slot_stride + (D / 8) * g;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = (r & 1) + 8 * (r >> 1);  // tokens 2j, 2j + 1, 2j + 8, 2j + 9
+            if (id >= 0) {
+              load_words<VW>(p + (long)row * pool.slot_stride, vw[s][r]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < VW; ++c) vw[s][r][c] = 0u;
+            }
+          }
+        }
+      };
+      uint32_t kw[ST][2][KW], vw[ST][4][VW];
+      int t = t_seg0 + w_off;
+      if (t < t_seg1) {
+        key_words(t, kw);
+        value_words(t, vw);
+      }
+      for (; t < t_seg1; t += TT) {
+        // scores of WT tokens x RT rows
+        float s[ST][NT][4];
+#pragma unroll
+        for (int u = 0; u < ST; ++u)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[dt][nt][i] = 0.f;
+            for (int i = 0; i < 4; ++i) s[u][nt][i] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
-        float vref = 0.f;
-
-        const int pg_end = (t_end + page_mask) >> lg;  // pages of the piece
-        for (int pg0 = t_begin >> lg; pg0 < pg_end; ) {
-          // ---- page ids and scales of the next pages (whole tiles)
-          const int t_seg0 = max(t_begin, pg0 << lg);
-          int t_seg1 = t_seg0 + (((pg0 + kSegPages) << lg) - t_seg0) / TT * TT;
-          t_seg1 = min(t_seg1, t_end);
-          const int np = ((t_seg1 + page_mask) >> lg) - pg0;
-          __syncthreads();  // the previous segment's (or unit's) readers are done
-          float vmax = 0.f;
-          for (int i = tid; i < np; i += kRowThreads) {
-            int id = a.table[(long)b * a.table_stride + pg0 + i];
-            if (id < 0 || id >= pool.num_pages) {
-              pool.flag(kStatusBounds, kPagedBadPage);
-              id = -1;
+        for (int u = 0; u < ST; ++u) {
+#pragma unroll
+          for (int kk = 0; kk < KW; ++kk) {
+            uint32_t f[4];
+            codes_to_f16<STORE>(kw[u][0][kk], &f[0], &f[2]);
+            codes_to_f16<STORE>(kw[u][1][kk], &f[1], &f[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(s[u][nt], f, qf[nt][kk][0], qf[nt][kk][1]);
+              if constexpr (SPLIT) mma_f16(s[u][nt], f, ql[nt][kk][0], ql[nt][kk][1]);
             }
-            seg_id[i] = id;
-            const float ks = id < 0 ? 0.f : pool.ks[(long)id * pool.scale_stride + h], vs = id < 0 ? 0.f : pool.vs[(long)id * pool.scale_stride + h];
-            seg_ks[i] = ks;
-            seg_w[i] = vs;
-            vmax = fmaxf(vmax, vs);
           }
-          vmax = warp_max(vmax);
-          if (lane == 0) red[warp] = vmax;
-          __syncthreads();
-          vmax = fmaxf(vref, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-          if (vmax > vref) {
-            if (vref > 0.f) {
-              const float r = vref / vmax;
+        }
+        float ksc[ST], vsc[ST], lvs[ST];
+        bool whole = t >= lo_all && t + WT <= hi_all;  // every row sees every token of the tile
+        bool bad[ST];
 #pragma unroll
-              for (int dt = 0; dt < D / 16; ++dt)
+        for (int u = 0; u < ST; ++u) {
+          const int pi = min(((t + 16 * u) >> lg) - pg0, np - 1);
+          ksc[u] = seg_ks[pi];
+          vsc[u] = seg_vs[pi];
+          lvs[u] = seg_lv[pi];
+          bad[u] = ((t + 16 * u) >> lg) - pg0 >= np || seg_id[pi] < 0;
+          whole = whole && !bad[u];
+        }
+        if (t + TT < t_seg1) key_words(t + TT, kw);
+        // maxima of x and of x + log2(vs), of this lane's tokens
+        float mt[NT][2], vt[NT][2];
+        bool grew = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) mt[nt][0] = mt[nt][1] = vt[nt][0] = vt[nt][1] = -INFINITY;
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[dt][nt][i] *= r;
-            }
-            vref = vmax;
-          }
-          const float inv_vref = vref > 0.f ? 1.f / vref : 0.f;
-
-          // ---- this warp's tiles
-          const int w_off = warp * WT;
-          auto key_words = [&](int t, uint32_t (&kw)[ST][2][KW]) {
+        for (int u = 0; u < ST; ++u) {
 #pragma unroll
-            for (int s = 0; s < ST; ++s) {
-              const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
-              const int id = pi < np ? seg_id[pi] : -1;
-              const unsigned char* p = pool.k + (long)id * pool.page_stride + (long)h * pool.head_stride +
-                                       (long)((tb & page_mask) + g) * pool.slot_stride + (D == 32 ? 8 : 16) * j;
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                if (id >= 0) {
-                  constexpr int W = KW < 4 ? KW : 4;
-#pragma unroll
-                  for (int c = 0; c < KW / W; ++c) load_words<W>(p + 8L * r * pool.slot_stride + 64 * c, &kw[s][r][W * c]);
-                } else {
-#pragma unroll
-                  for (int c = 0; c < KW; ++c) kw[s][r][c] = 0u;
-                }
-              }
-            }
-          };
-          auto value_words = [&](int t, uint32_t (&vw)[ST][4][VW]) {
-#pragma unroll
-            for (int s = 0; s < ST; ++s) {
-              const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
-              const int id = pi < np ? seg_id[pi] : -1;
-              const unsigned char* p = pool.v + (long)id * pool.page_stride + (long)h * pool.head_stride +
-                                       (long)((tb & page_mask) + 2 * j) * pool.slot_stride + (D / 8) * g;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int row = (r & 1) + 8 * (r >> 1);  // tokens 2j, 2j + 1, 2j + 8, 2j + 9
-                if (id >= 0) {
-                  load_words<VW>(p + (long)row * pool.slot_stride, vw[s][r]);
-                } else {
-#pragma unroll
-                  for (int c = 0; c < VW; ++c) vw[s][r][c] = 0u;
-                }
-              }
-            }
-          };
-          uint32_t kw[ST][2][KW], vw[ST][4][VW];
-          int t = t_seg0 + w_off;
-          if (t < t_seg1) {
-            key_words(t, kw);
-            value_words(t, vw);
-          }
-          for (; t < t_seg1; t += TT) {
-            // scores of WT tokens x RT rows
-            float s[ST][NT][4];
-#pragma unroll
-            for (int u = 0; u < ST; ++u)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[u][nt][i] = 0.f;
-#pragma unroll
-            for (int u = 0; u < ST; ++u) {
-#pragma unroll
-              for (int kk = 0; kk < KW; ++kk) {
-                uint32_t f[4];
-                codes_to_f16<STORE>(kw[u][0][kk], &f[0], &f[2]);
-                codes_to_f16<STORE>(kw[u][1][kk], &f[1], &f[3]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  mma_f16(s[u][nt], f, qf[nt][kk][0], qf[nt][kk][1]);
-                  if constexpr (SPLIT) mma_f16(s[u][nt], f, ql[nt][kk][0], ql[nt][kk][1]);
-                }
-              }
-            }
-            float ksc[ST], vsc[ST];
-#pragma unroll
-            for (int u = 0; u < ST; ++u) {
-              const int pi = min(((t + 16 * u) >> lg) - pg0, np - 1);
-              ksc[u] = seg_ks[pi];
-              vsc[u] = seg_w[pi] * inv_vref;
-            }
-            if (t + TT < t_seg1) key_words(t + TT, kw);
-            bool whole = t >= lo_all && t + WT <= hi_all;  // every row sees every token of the tile
-#pragma unroll
-            for (int u = 0; u < ST; ++u) {
-              const int pi = ((t + 16 * u) >> lg) - pg0;
-              whole = whole && pi < np && seg_id[pi] >= 0;
-            }
-            float mt[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mt[nt][0] = m[nt][0], mt[nt][1] = m[nt][1];
-#pragma unroll
-            for (int u = 0; u < ST; ++u) {
-              const bool bad = !whole && (((t + 16 * u) >> lg) - pg0 >= np || seg_id[((t + 16 * u) >> lg) - pg0] < 0);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const float c0 = ksc[u] * cq[nt][0], c1 = ksc[u] * cq[nt][1];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  s[u][nt][i] *= (i & 1) ? c1 : c0;
-                  if (!whole) {
-                    const int tok = t + 16 * u + g + 8 * (i >> 1);
-                    if (bad || tok < lim_lo[nt][i & 1] || tok >= lim_hi[nt][i & 1]) s[u][nt][i] = -INFINITY;
-                  }
-                  mt[nt][i & 1] = fmaxf(mt[nt][i & 1], s[u][nt][i]);
-                }
-              }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) mt[nt][c] = fmaxf(mt[nt][c], __shfl_xor_sync(0xffffffffu, mt[nt][c], o));
-              }
-            bool grew = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) grew |= mt[nt][0] > m[nt][0] || mt[nt][1] > m[nt][1];
-            if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float al[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  al[c] = m[nt][c] == -INFINITY ? 0.f : exp2_fast(m[nt][c] - mt[nt][c]);
-                  l[nt][c] *= al[c];
-                  m[nt][c] = mt[nt][c];
-                }
-#pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[dt][nt][i] *= al[i & 1];
-              }
-            }
-            // weights, rounded to f16 after the page's value scale, as the B operand
-            uint32_t pf[ST][NT][2], pl[SPLIT ? ST : 1][SPLIT ? NT : 1][2];
-#pragma unroll
-            for (int u = 0; u < ST; ++u)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < 2; ++c) {
+              const float f = ksc[u] * cq[nt][c];
+              s[u][nt][c] *= f;
+              s[u][nt][2 + c] *= f;
+              if (!whole) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                  float p[2];
-#pragma unroll
-                  for (int c = 0; c < 2; ++c) {
-                    const float base = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-                    p[c] = exp2_fast(s[u][nt][2 * hf + c] - base);
-                    l[nt][c] += p[c];
-                    p[c] *= vsc[u];
-                  }
-                  const uint32_t w = pack_f16(p[0], p[1]);
-                  pf[u][nt][hf] = transpose_f16x2(w);
-                  if constexpr (SPLIT) {
-                    const float2 r = unpack_f16(w);
-                    pl[u][nt][hf] = transpose_f16x2(pack_f16(p[0] - r.x, p[1] - r.y));
-                  }
-                }
-            if (!whole) {  // codes of tokens outside [lo, hi) may be anything
-#pragma unroll
-              for (int u = 0; u < ST; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int tok = t + 16 * u + 2 * j + (r & 1) + 8 * (r >> 1);
-                  if (tok < lo || tok >= hi) {
-#pragma unroll
-                    for (int c = 0; c < VW; ++c) vw[u][r][c] = 0u;
-                  }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < ST; ++u)
-#pragma unroll
-              for (int c = 0; c < VW; ++c) {
-                // words c of tokens 2j, 2j+1 (then 2j+8, 2j+9): dims 4c .. 4c+3 of the lane's chunk
-                const uint32_t p01 = __byte_perm(vw[u][0][c], vw[u][1][c], 0x5140);
-                const uint32_t p23 = __byte_perm(vw[u][0][c], vw[u][1][c], 0x7362);
-                const uint32_t r01 = __byte_perm(vw[u][2][c], vw[u][3][c], 0x5140);
-                const uint32_t r23 = __byte_perm(vw[u][2][c], vw[u][3][c], 0x7362);
-                uint32_t f[4], e[4];
-                codes_to_f16<STORE>(p01, &f[0], &f[1]);
-                codes_to_f16<STORE>(r01, &f[2], &f[3]);
-                codes_to_f16<STORE>(p23, &e[0], &e[1]);
-                codes_to_f16<STORE>(r23, &e[2], &e[3]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  mma_f16(acc[2 * c][nt], f, pf[u][nt][0], pf[u][nt][1]);
-                  mma_f16(acc[2 * c + 1][nt], e, pf[u][nt][0], pf[u][nt][1]);
-                  if constexpr (SPLIT) {
-                    mma_f16(acc[2 * c][nt], f, pl[u][nt][0], pl[u][nt][1]);
-                    mma_f16(acc[2 * c + 1][nt], e, pl[u][nt][0], pl[u][nt][1]);
-                  }
+                  const int tok = t + 16 * u + g + 8 * hf;
+                  if (bad[u] || tok < lim_lo[nt][c] || tok >= lim_hi[nt][c]) s[u][nt][2 * hf + c] = -INFINITY;
                 }
               }
-            if (t + TT < t_seg1) value_words(t + TT, vw);
+              const float x = fmaxf(s[u][nt][c], s[u][nt][2 + c]);
+              mt[nt][c] = fmaxf(mt[nt][c], x);
+              vt[nt][c] = fmaxf(vt[nt][c], x + lvs[u]);
+            }
           }
-          pg0 = t_seg1 >> lg;  // a tile border is a page border, or the end of the piece
-          if (t_seg1 >= t_end) break;
         }
-
-        // ---- the four warps' shares: one maximum, summed accumulators
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c) grew |= mt[nt][c] > m[nt][c] + 8.f || vt[nt][c] > mv[nt][c] + 8.f;
+        if (__any_sync(0xffffffffu, grew)) {  // rare after the first tiles
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
-            if (g == 0) {
-              sm_m[warp][8 * nt + 2 * j + c] = m[nt][c];
-              sm_l[warp][8 * nt + 2 * j + c] = l[nt][c];
+          for (int nt = 0; nt < NT; ++nt) {
+            float al[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = fmaxf(m[nt][c], mt[nt][c]), y = fmaxf(mv[nt][c], vt[nt][c]);
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+              }
+              if (m[nt][c] != -INFINITY) l[nt][c] *= exp2_fast(m[nt][c] - x);
+              al[c] = mv[nt][c] == -INFINITY ? 1.f : exp2_fast(mv[nt][c] - y);
+              m[nt][c] = x;
+              mv[nt][c] = y;
             }
-          }
-        __syncthreads();
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int r = 8 * nt + 2 * j + c;
-            const float M = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
-            // a warp that saw nothing has O = 0 (or NaN, from a NaN query)
-            const float f = m[nt][c] == -INFINITY ? 1.f : exp2_fast(m[nt][c] - M);
-            float* dst = osm + ((long)warp * RT + r) * D + (D / 8) * g;
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) {
-              dst[2 * dt] = acc[dt][nt][c] * f;
-              dst[2 * dt + 1] = acc[dt][nt][2 + c] * f;
-            }
-          }
-        __syncthreads();
-        const bool whole_unit = off == 0 && n_here == span;
-        float* rec = a.part.rec + ((long)blockIdx.x * 2 + (off == 0 ? 1 : 0)) * RT * (D + 2);
-        for (int e = tid; e < RT * D; e += kRowThreads) {
-          const int r = e / D, d = e % D, R = row0 + r;
-          if (R >= rows) break;
-          const float M = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
-          float L = 0.f, o = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            L += sm_l[w][r] * (sm_m[w][r] == -INFINITY ? 1.f : exp2_fast(sm_m[w][r] - M));
-            o += osm[(w * RT + r) * D + d];
-          }
-          o *= vref;
-          if (whole_unit) {
-            const long row = (rq.cu_q ? rq.q0(b) : (long)b * rq.q_tokens) + R / rq.G;
-            const int hq = h * rq.G + R % rq.G;
-            store_f(reinterpret_cast<T*>(a.out.out) + (row * a.out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
-            if (d == 0 && a.out.lse)
-              a.out.lse[row * a.out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
-          } else {
-            rec[r * D + d] = o;
-            if (d == 0) {
-              rec[RT * D + r] = M;
-              rec[RT * D + RT + r] = L;
-            }
+              for (int i = 0; i < 4; ++i) acc[dt][nt][i] *= al[i & 1];
           }
         }
-        if (off == 0 && n_here < span) {  // begun here, finished by the CTAs that follow
-          const long rest = span - n_here;
-          begun = make_int4(b, h, rt, 1 + (int)((rest + at.chunk - 1) / at.chunk));
+        // weights p vs / 2^(mv - m), rounded to f16, as the B operand
+        uint32_t pf[ST][NT][2], pl[SPLIT ? ST : 1][SPLIT ? NT : 1][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float base[2], fr[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            base[c] = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+            fr[c] = mv[nt][c] == -INFINITY ? 0.f : exp2_fast(m[nt][c] - mv[nt][c]);
+          }
+#pragma unroll
+          for (int u = 0; u < ST; ++u)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              float p[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                p[c] = exp2_fast(s[u][nt][2 * hf + c] - base[c]);
+                l[nt][c] += p[c];
+                p[c] *= fminf(vsc[u] * fr[c], 0x1p100f);
+              }
+              const uint32_t w = pack_f16(p[0], p[1]);
+              pf[u][nt][hf] = transpose_f16x2(w);
+              if constexpr (SPLIT) {
+                const float2 r = unpack_f16(w);
+                pl[u][nt][hf] = transpose_f16x2(pack_f16(p[0] - r.x, p[1] - r.y));
+              }
+            }
         }
-        left -= n_here;
-        __syncthreads();  // the output's readers are done
+        if (!whole) {  // codes of tokens outside [lo, hi) may be anything
+#pragma unroll
+          for (int u = 0; u < ST; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int tok = t + 16 * u + 2 * j + (r & 1) + 8 * (r >> 1);
+              if (tok < lo || tok >= hi) {
+#pragma unroll
+                for (int c = 0; c < VW; ++c) vw[u][r][c] = 0u;
+              }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < ST; ++u)
+#pragma unroll
+          for (int c = 0; c < VW; ++c) {
+            // words c of tokens 2j, 2j+1 (then 2j+8, 2j+9): dims 4c .. 4c+3 of the lane's chunk
+            const uint32_t p01 = __byte_perm(vw[u][0][c], vw[u][1][c], 0x5140);
+            const uint32_t p23 = __byte_perm(vw[u][0][c], vw[u][1][c], 0x7362);
+            const uint32_t r01 = __byte_perm(vw[u][2][c], vw[u][3][c], 0x5140);
+            const uint32_t r23 = __byte_perm(vw[u][2][c], vw[u][3][c], 0x7362);
+            uint32_t f[4], e[4];
+            codes_to_f16<STORE>(p01, &f[0], &f[1]);
+            codes_to_f16<STORE>(r01, &f[2], &f[3]);
+            codes_to_f16<STORE>(p23, &e[0], &e[1]);
+            codes_to_f16<STORE>(r23, &e[2], &e[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(acc[2 * c][nt], f, pf[u][nt][0], pf[u][nt][1]);
+              mma_f16(acc[2 * c + 1][nt], e, pf[u][nt][0], pf[u][nt][1]);
+              if constexpr (SPLIT) {
+                mma_f16(acc[2 * c][nt], f, pl[u][nt][0], pl[u][nt][1]);
+                mma_f16(acc[2 * c + 1][nt], e, pl[u][nt][0], pl[u][nt][1]);
+              }
+            }
+          }
+        if (t + TT < t_seg1) value_words(t + TT, vw);
       }
-      off = 0;
+      pg0 = t_seg1 >> lg;  // a tile border is a page border, or the end of the piece
+      if (t_seg1 >= t_end) break;
     }
-    ++b;
+
+    // ---- the four warps' shares: one maximum, summed accumulators
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+        if (g == 0) {
+          sm_m[warp][8 * nt + 2 * j + c] = m[nt][c];
+          sm_l[warp][8 * nt + 2 * j + c] = l[nt][c];
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = 8 * nt + 2 * j + c;
+        const float M = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
+        // a warp that saw nothing has O = 0 (or NaN, from a NaN query)
+        const float f = mv[nt][c] == -INFINITY ? 1.f : exp2_fast(mv[nt][c] - M);
+        float* dst = osm + ((long)warp * RT + r) * D + (D / 8) * g;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          dst[2 * dt] = acc[dt][nt][c] * f;
+          dst[2 * dt + 1] = acc[dt][nt][2 + c] * f;
+        }
+      }
+    __syncthreads();
+    const bool whole_unit = pc.whole();
+    float* rec = a.part.rec + ((long)blockIdx.x * 2 + (pc.off == 0 ? 1 : 0)) * RT * (D + 2);
+    for (int e = tid; e < RT * D; e += kRowThreads) {
+      const int r = e / D, d = e % D, R = row0 + r;
+      if (R >= rows) break;
+      const float M = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
+      float L = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        L += sm_l[w][r] * (sm_m[w][r] == -INFINITY ? 1.f : exp2_fast(sm_m[w][r] - M));
+        o += osm[(w * RT + r) * D + d];
+      }
+      if (whole_unit) {
+        const long row = pc.out_row(R);
+        const int hq = h * rq.G + R % rq.G;
+        store_f(reinterpret_cast<T*>(a.out.out) + (row * a.out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
+        if (d == 0 && a.out.lse)
+          a.out.lse[row * a.out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+      } else {
+        rec[r * D + d] = o;
+        if (d == 0) {
+          rec[RT * D + r] = M;
+          rec[RT * D + RT + r] = L;
+        }
+      }
+    }
+    if (const int n = pc.pieces(at.chunk)) begun = make_int4(b, h, pc.rt, n);
+    __syncthreads();  // the output's readers are done
   }
   if (tid == 0) a.part.head[blockIdx.x] = begun;
-}
-
-// Joins a split unit's records: M = max m_i, out = sum 2^(m_i - M) O_i / sum
-// 2^(m_i - M) l_i.  One CTA per (CTA of the kernel above, slice of the rows);
-// most have nothing to do.  Bound by the latency of reading the records.
-template <int D, int RT, typename T>
-__global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPart part, PagedOut out, int fill_tail) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (fill_tail && rq.cu_q) {  // rows behind the last request: zeros
-    const long from = (long)max(0, min(rq.cu_q[rq.batch], rq.q_tokens)) * out.Hq, to = (long)rq.q_tokens * out.Hq;
-    const long stride = (long)gridDim.x * gridDim.y * 128;
-    const long at = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + threadIdx.x;
-    for (long e = from * D + at; e < to * D; e += stride) store_f(reinterpret_cast<T*>(out.out) + e, 0.f);
-    if (out.lse)
-      for (long e = from + at; e < to; e += stride) out.lse[e] = -INFINITY;
-  }
-  const int4 u = part.head[blockIdx.x];
-  if (u.w == 0) return;
-  const int b = u.x, h = u.y, rt = u.z, n = u.w;
-  const int rows = min(RT, rq.q_len(b) * rq.G - rt * RT);
-  const long step = 2L * RT * (D + 2);
-  const float* r0 = part.rec + (long)blockIdx.x * step + (long)RT * (D + 2);  // record 1 of the first CTA
-  const float* r1 = part.rec + (long)(blockIdx.x + 1) * step;                 // record 0 of those after it
-  for (int e = blockIdx.y * 128 + threadIdx.x; e < rows * D; e += gridDim.y * 128) {
-    const int r = e / D, d = e % D;
-    float M = r0[RT * D + r];
-#pragma unroll 8
-    for (int i = 0; i < n - 1; ++i) M = fmaxf(M, r1[i * step + RT * D + r]);
-    const float f = M == -INFINITY ? 1.f : exp2_fast(r0[RT * D + r] - M);
-    float L = f * r0[RT * D + RT + r], o = f * r0[r * D + d];
-#pragma unroll 8
-    for (int i = 0; i < n - 1; ++i) {
-      const float* p = r1 + i * step;
-      const float w = M == -INFINITY ? 1.f : exp2_fast(p[RT * D + r] - M);
-      L = fmaf(w, p[RT * D + RT + r], L);
-      o = fmaf(w, p[r * D + d], o);
-    }
-    const int R = rt * RT + r;
-    const long row = (rq.cu_q ? rq.q0(b) : (long)b * rq.q_tokens) + R / rq.G;
-    const int hq = h * rq.G + R % rq.G;
-    store_f(reinterpret_cast<T*>(out.out) + (row * out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
-    if (d == 0 && out.lse) out.lse[row * out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
-  }
 }
 
 }  // namespace kvd
@@ -605,39 +522,14 @@ int paged_pool_view(const kvd_paged_pool* p, PagedPool* out) {
   return KVD_OK;
 }
 
+// A request of at most this many rows goes to the few-row kernel: its codes are
+// read once per 8 or 16 rows, the tensor-memory kernel's once per 256.
+constexpr int kFewRows = 32;
+
 // rows per unit of the few-row kernel: eight, or sixteen for longer groups
 // (head_dim 256: sixteen rows' accumulators would not fit the registers)
 static int rows_nt(long max_rows, int D) { return max_rows <= 8 || D == 256 ? 1 : 2; }
 static int rows_ctas(int D, int nt, bool fp32) { return paged_sm_count() * rows_per_sm(D, nt, fp32); }
-
-static size_t part_bytes(int ctas, int rt, int D) {
-  return (size_t)ctas * sizeof(int4) + (size_t)ctas * 2 * rt * (D + 2) * sizeof(float);
-}
-static PagedPart part_at(void* ws, int ctas) {
-  PagedPart p;
-  p.head = (int4*)ws;
-  p.rec = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
-  return p;
-}
-
-template <int D, int RT, typename T>
-static int launch_merge(const PagedReqs& rq, const PagedPart& part, const PagedOut& out, int fill_tail, int ctas,
-                        cudaStream_t s) {
-  // starts while the kernel before it drains, and waits for it in the kernel
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, (RT * D + 511) / 512);
-  cfg.blockDim = dim3(128);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  KTimerScope kts_("paged_merge_kernel", s);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, RT, T>, rq, part, out, fill_tail);
-  if (e != cudaSuccess) { set_error("paged_merge_kernel: %s", cudaGetErrorString(e)); return KVD_ERR_CUDA; }
-  return KVD_OK;
-}
 
 template <int D, int NT, int STORE, typename T>
 static int launch_rows(RowArgs& a, void* ws, cudaStream_t s) {
@@ -684,6 +576,7 @@ extern "C" size_t kvd_paged_attention_workspace_bytes(const kvd_paged_pool* pool
   const int D = pool->head_dim;
   size_t need = 0;
   for (int nt = 1; nt <= 2; ++nt) need = std::max(need, part_bytes(rows_ctas(D, nt, dtype == KVD_DTYPE_F32), 8 * nt, D));
+  if (paged_chunk_takes(D, dtype)) need = std::max(need, paged_chunk_ws_bytes(D));
   return need;
 }
 
@@ -722,7 +615,21 @@ extern "C" int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, co
   a.scaling = scaling * 1.4426950408889634f;
   a.out.out = out; a.out.lse = lse; a.out.Hq = num_q_heads;
   const int most = cu_q ? std::min(max_q > 0 ? max_q : q_tokens, q_tokens) : q_tokens;
-  const int nt = rows_nt((long)most * G, D);
+  // Requests of more rows than kFewRows go to the tensor-memory kernel, where it
+  // takes the shape; a packed batch may hold both kinds, and each kernel passes
+  // over the other's requests.  One workspace serves both: they run in turn.
+  const bool chunks = paged_chunk_takes(D, dtype) && (long)most * G > kFewRows;
+  const bool few = !chunks || cu_q;
+  if (chunks) {
+    PagedReqs rc_ = r;
+    rc_.min_rows = kFewRows + 1;
+    if (int rc = launch_paged_chunk(a.pool, D, pool->store, rc_, table, table_stride, dtype, q, q_sb, q_sh, q_st, a.scaling, a.out,
+                                    few ? 0 : fill_tail, workspace, (cudaStream_t)stream))
+      return rc;
+    r.max_rows = kFewRows;
+  }
+  if (!few) return KVD_OK;
+  const int nt = rows_nt(std::min((long)most * G, (long)r.max_rows), D);
   if (dtype == KVD_DTYPE_F32) return launch_rows_t<float>(a, D, nt, pool->store, workspace, (cudaStream_t)stream);
   if (dtype == KVD_DTYPE_BF16) return launch_rows_t<__nv_bfloat16>(a, D, nt, pool->store, workspace, (cudaStream_t)stream);
   return launch_rows_t<__half>(a, D, nt, pool->store, workspace, (cudaStream_t)stream);
