@@ -337,7 +337,7 @@ int kvd_paged_peek(const kvd_paged_pool* pool, int32_t batch, const int32_t* tab
  * starts may be NULL) and, with window > 0, t > lens[b] - n + i - window.  A
  * row that sees nothing gives zeros and lse -inf.  cu_q [batch + 1] (packed
  * queries, q_tokens rows in all, max_q the most of one request or 0 for not
- * known) or NULL (every request has q_tokens).  q: element strides of batch,
+ * known) or NULL (every request has q_tokens).  scaling > 0; scales > 0 or 0.  q: element strides of batch,
  * head and token, multiples of 16 bytes, unit stride over D.  out
  * (rows, num_q_heads, D) contiguous, lse (rows, num_q_heads) or NULL: natural
  * log of the softmax sum.  Rows behind cu_q[batch] are left as they were, or

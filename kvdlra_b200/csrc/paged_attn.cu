@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float f = ksc[u] * cq[nt][c];
+              const float f = fmaxf(ksc[u] * cq[nt][c], 0x1p-126f);
               s[u][nt][c] *= f;
               s[u][nt][2 + c] *= f;
               if (!whole) {
@@ -591,6 +591,7 @@ extern "C" int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, co
   if (dtype != KVD_DTYPE_F32 && dtype != KVD_DTYPE_BF16 && dtype != KVD_DTYPE_F16) { set_error("paged attention: unsupported dtype %d", dtype); return KVD_ERR_DTYPE; }
   if (batch < 0 || q_tokens < 0 || max_q < 0 || max_pages < 0 || window < 0 || table_stride < max_pages) { set_error("paged attention: negative size, or a table stride below its width"); return KVD_ERR_ARG; }
   if (num_q_heads < H || num_q_heads % H) { set_error("paged attention: %d query heads over %d KV heads", num_q_heads, H); return KVD_ERR_ARG; }
+  if (!(scaling > 0.f) || scaling > 1e30f) { set_error("paged attention: scaling must be positive and finite, got %g", scaling); return KVD_ERR_ARG; }
   if (batch == 0 || q_tokens == 0) return KVD_OK;
   const int G = num_q_heads / H;
   if ((int64_t)q_tokens * G > INT32_MAX / 2 || (int64_t)max_pages * pool->page_size > INT32_MAX / 2) { set_error("paged attention: too many rows or cached tokens for one request"); return KVD_ERR_ARG; }

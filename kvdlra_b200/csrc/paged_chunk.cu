@@ -6,16 +6,15 @@
 // 128-token tile:
 //   loaders (4 warps)  the page's codes from global memory, a tile ahead in
 //                      registers, converted exactly to f16 and written to shared
-//                      memory in the no-swizzle core-matrix layout.  The image
-//                      [token / 8][dim / 8][token % 8][16 bytes] serves keys as a
-//                      K-major and values as an MN-major operand.
+//                      memory as rows of 64 dims with the 128-byte swizzle: the
+//                      same image is a K-major operand of the scores and an
+//                      MN-major one of the values.
 //   issuer (1 thread)  S_w = Q_w K^T for the two row tiles w of 128 rows, and
 //                      O_w += P_w V with P_w in TMEM; while one row tile's
 //                      softmax runs, the tensor core works for the other.
 //   softmax (2 x 4 warps)  a thread owns a row (a TMEM lane): the row's maxima
-//                      and sums need no other thread.  S is read twice, once for
-//                      the maximum and once for the weights; P_w (f16) goes over
-//                      the columns of S_w that were read.
+//                      and sums need no other thread.  P_w (f16) goes over the
+//                      columns of S_w.
 // TMEM: S_0, S_1 (128 columns each), O_0, O_1 (head_dim each).
 //
 // Two references per row, in base 2: m for the sum l of the weights, and mv
@@ -37,8 +36,13 @@
 namespace kvd {
 
 constexpr int kPcRows = 256, kPcTok = 128;
-constexpr int kPcThreads = 416;            // 8 softmax warps, 4 loaders, 1 issuer
-constexpr int kPcLoad0 = 256, kPcIssue0 = 384;
+constexpr int kPcThreads = 512;            // 8 softmax warps, 4 loaders, issuer, planner (and 2 that wait)
+// registers per thread of the four warpgroups: a softmax thread holds its row
+// of S, a loader a tile's codes; their sum is what the CTA is launched with
+constexpr int kPcRegsSoftmax = 168, kPcRegsLoad = 128, kPcRegsIssue = 48;
+static_assert(2 * kPcRegsSoftmax + kPcRegsLoad + kPcRegsIssue == 4 * (65536 / kPcThreads), "register split");
+constexpr int kPcLoad0 = 256, kPcIssue0 = 384, kPcPlan0 = 416;
+constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
 constexpr long kPcPolls = 1L << 20;
 
 struct ChunkArgs {
@@ -58,6 +62,17 @@ struct ChunkScales {  // of one tile, per 16 tokens
   int bad[8];                 // page id out of range
 };
 
+// A piece of the CTA's work, as the planner hands it to the other roles (their
+// registers have no room for the walk over the requests).
+struct ChunkPiece {
+  int n, tile;            // its token tiles; 0: there are no more pieces
+  int b, h, row0, rows;   // request, KV head, the unit's first row, rows of the request
+  int lo, hi;             // tokens that any of the unit's rows sees
+  int len, q_len, start, q0;
+  int whole, begins;      // covers its unit; begins it
+};
+constexpr int kPcPieces = 4;  // pieces planned ahead
+
 template <int D>
 struct ChunkSmem {
   static constexpr int NS = D == 64 ? 4 : 2;   // stages of keys, and of values
@@ -65,8 +80,8 @@ struct ChunkSmem {
   static constexpr int q = 0, v = q + 2 * tile, k = v + NS * tile, sc = k + NS * tile;
   static constexpr int ring = 8;               // tiles whose scales are held: NS + 1 at least
   static constexpr int bars = sc + ring * (int)sizeof(ChunkScales);
-  static constexpr int nbars = 4 * NS + 8;
-  static constexpr int total = bars + nbars * 8 + 16;
+  static constexpr int nbars = 4 * NS + 8 + 2 * kPcPieces;
+  static constexpr int total = bars + nbars * 8 + 1024;  // room to align
 };
 
 KVD_DEVICE uint64_t pack2(float a, float b) {
@@ -95,14 +110,17 @@ template <int D, int STORE, typename T>
 __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
   using L = ChunkSmem<D>;
   constexpr int NS = L::NS;
-  extern __shared__ __align__(1024) unsigned char psm[];
+  extern __shared__ unsigned char psm_raw[];
+  unsigned char* psm = psm_raw + (-(int)(uint32_t)__cvta_generic_to_shared(psm_raw) & 1023);  // swizzle atoms are aligned
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;  // a wait gave up
+  __shared__ ChunkPiece pieces[kPcPieces];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedPool& pool = a.pool;
   const PagedReqs& rq = a.reqs;
   uint64_t* bars = reinterpret_cast<uint64_t*>(psm + L::bars);
-  uint64_t *kf = bars, *ke = kf + NS, *vf = ke + NS, *ve = vf + NS, *sf = ve + NS, *pf = sf + 2, *of = pf + 2, *qf = of + 2, *drain = qf + 1;
+  uint64_t *kf = bars, *ke = kf + NS, *vf = ke + NS, *ve = vf + NS, *sf = ve + NS, *pf = sf + 2, *of = pf + 2, *qf = of + 2, *drain = qf + 1,
+           *nf = drain + 1, *ne = nf + kPcPieces;
   ChunkScales* scales = reinterpret_cast<ChunkScales*>(psm + L::sc);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
@@ -122,6 +140,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       umma::mbar_init(pf + w, 128);
       umma::mbar_init(of + w, 1);
     }
+    for (int i = 0; i < kPcPieces; ++i) {
+      umma::mbar_init(nf + i, 1);
+      umma::mbar_init(ne + i, 256 + 128 + 1);
+    }
     umma::mbar_init(qf, 256);
     umma::mbar_init(drain, 1);
     umma::mbar_fence_init();
@@ -130,7 +152,6 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   const WorkAt at = find_work<kPcRows, kPcTok, kPcThreads>(rq, blockIdx.x, gridDim.x);  // has barriers
   umma::fence_after_sync();
   const uint32_t tmem = tmem_base;
-  Pieces<kPcRows, kPcTok> pc(rq, at, blockIdx.x);
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     for (long i = 0; i < kPcPolls; ++i) {
       if (umma::mbar_try_wait(bar, parity)) return true;
@@ -140,85 +161,146 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     pool.flag(kStatusTimeout, 1);
     return false;
   };
-  int4 begun = make_int4(0, 0, 0, 0);
 
   if (tid >= kPcIssue0) {
-    // ------------------------------------------------------------ issuer
-    if (lane == 0) {
-      const uint32_t q_a = (uint32_t)__cvta_generic_to_shared(psm + L::q);
-      const uint32_t k_a = (uint32_t)__cvta_generic_to_shared(psm + L::k);
-      const uint32_t v_a = (uint32_t)__cvta_generic_to_shared(psm + L::v);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcRegsIssue));
+    if (warp == kPcPlan0 / 32 && lane == 0) {
+      // ---------------------------------------------------------- planner
+      Pieces<kPcRows, kPcTok> pc(rq, at, blockIdx.x);
+      int4 begun = make_int4(0, 0, 0, 0);
+      for (int k = 0;; ++k) {
+        const bool more = pc.next();
+        const int sl = k % kPcPieces;
+        if (!wait(ne + sl, ((k / kPcPieces) & 1) ^ 1)) break;
+        ChunkPiece& p = pieces[sl];
+        p.n = more ? pc.n : 0;
+        if (more) {
+          p.tile = pc.tile; p.b = pc.b; p.h = pc.h; p.row0 = pc.rt * kPcRows; p.rows = pc.rows;
+          p.lo = pc.lo; p.hi = pc.hi; p.len = pc.len; p.q_len = pc.q_len; p.start = pc.start; p.q0 = rq.q0(pc.b);
+          p.whole = pc.whole(); p.begins = pc.off == 0;
+          if (const int n = pc.pieces(at.chunk)) begun = make_int4(pc.b, pc.h, pc.rt, n);
+        }
+        umma::mbar_arrive(nf + sl);
+        if (!more) break;
+      }
+      a.part.head[blockIdx.x] = begun;
+    } else if (warp == kPcIssue0 / 32) {
+      // ----------------------------------------------------------- issuer
+      // the whole warp walks, one lane issues: descriptors stay in uniform registers
+      const uint64_t q_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::q), 16, 1024);
+      const uint64_t k_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::k), 16, 1024);
+      const uint64_t v_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::v), kPcBlock, 1024);
       constexpr uint32_t id_s = umma::idesc_f16(128, kPcTok, false), id_o = umma::idesc_f16(128, D, true);
+      // a descriptor's address field counts 16 bytes
       auto scores = [&](int w, int stage) {
+        const uint64_t q_w = q_d + w * (L::tile >> 4), k_s = k_d + stage * (L::tile >> 4);
+        if (umma::elect_one()) {
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-          umma::mma_bf16(tmem + 128 * w, umma::smem_desc(q_a + w * L::tile + 256 * j, 128, 16 * D),
-                         umma::smem_desc(k_a + stage * L::tile + 256 * j, 128, 16 * D), id_s, j > 0);
-      };
-      auto values = [&](int w, int stage, bool acc) {
-#pragma unroll
-        for (int j = 0; j < kPcTok / 16; ++j)
-          umma::mma_f16_ts(tmem + 256 + D * w, tmem + 128 * w + 8 * j,
-                           umma::smem_desc(v_a + stage * L::tile + 32 * D * j, 16 * D, 128), id_o, acc || j > 0);
-      };
-      int it = 0, un = 0, tc[2] = {0, 0};
-      bool ok = true;
-      while (ok && pc.next()) {
-        const int nw = pc.rows - pc.rt * kPcRows > 128 ? 2 : 1;
-        ok = wait(qf, un & 1) && wait(kf + it % NS, (it / NS) & 1);
-        if (!ok) break;
-        umma::fence_after_sync();
-        for (int w = 0; w < nw; ++w) {
-          scores(w, it % NS);
+          for (int j = 0; j < D / 16; ++j) {
+            const uint64_t at_j = ((j >> 2) * kPcBlock + 32 * (j & 3)) >> 4;
+            umma::mma_bf16(tmem + 128 * w, q_w + at_j, k_s + at_j, id_s, j > 0);
+          }
           umma::commit(sf + w);
         }
-        umma::commit(ke + it % NS);
-        for (int i = 0; i < pc.n && ok; ++i) {
+        __syncwarp();
+      };
+      auto values = [&](int w, int stage, bool acc) {
+        const uint64_t v_s = v_d + stage * (L::tile >> 4);
+        if (umma::elect_one()) {
+#pragma unroll
+          for (int j = 0; j < kPcTok / 16; ++j)
+            umma::mma_f16_ts(tmem + 256 + D * w, tmem + 128 * w + 8 * j, v_s + ((2048 * j) >> 4), id_o, acc || j > 0);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (umma::elect_one()) umma::commit(bar);
+        __syncwarp();
+      };
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
+      int it = 0, tc0 = 0, tc1 = 0;
+      bool ok = true;
+      for (int un = 0;; ++un) {
+        const int sl = un % kPcPieces;
+        ok = wait_all(nf + sl, (un / kPcPieces) & 1);
+        if (!ok) break;
+        const int n = __shfl_sync(0xffffffffu, pieces[sl].n, 0);
+        const bool two = __shfl_sync(0xffffffffu, pieces[sl].rows - pieces[sl].row0 > 128, 0);
+        if (lane == 0) umma::mbar_arrive(ne + sl);
+        if (n == 0) break;
+        ok = wait_all(qf, un & 1) && wait_all(kf + it % NS, (it / NS) & 1);
+        if (!ok) break;
+        umma::fence_after_sync();
+        scores(0, it % NS);
+        if (two) scores(1, it % NS);
+        commit(ke + it % NS);
+        for (int i = 0; i < n; ++i) {
           const int g = it + i, st = g % NS, nx = (g + 1) % NS;
-          ok = wait(vf + st, (g / NS) & 1);
-          for (int w = 0; w < nw && ok; ++w) {
-            ok = wait(pf + w, tc[w] & 1);
+          const bool more = i + 1 < n;
+          ok = wait_all(vf + st, (g / NS) & 1) && wait_all(pf, tc0++ & 1);
+          if (!ok) break;
+          umma::fence_after_sync();
+          values(0, st, i > 0);
+          if (!two) commit(ve + st);
+          if (more) {
+            ok = wait_all(kf + nx, ((g + 1) / NS) & 1);
             if (!ok) break;
-            ++tc[w];
             umma::fence_after_sync();
-            values(w, st, i > 0);
-            if (w == nw - 1) umma::commit(ve + st);
-            if (i + 1 < pc.n) {
-              if (w == 0) ok = wait(kf + nx, ((g + 1) / NS) & 1);
-              if (!ok) break;
-              umma::fence_after_sync();
-              // S_w over P_w: the tensor core takes this thread's products in order
-              scores(w, nx);
-              umma::commit(sf + w);
-              if (w == nw - 1) umma::commit(ke + nx);
-            } else {
-              umma::commit(of + w);
-            }
+            scores(0, nx);  // S over P: the tensor core takes one thread's products in order
+            if (!two) commit(ke + nx);
+          } else {
+            commit(of);
+          }
+          if (!two) continue;
+          ok = wait_all(pf + 1, tc1++ & 1);
+          if (!ok) break;
+          umma::fence_after_sync();
+          values(1, st, i > 0);
+          commit(ve + st);
+          if (more) {
+            scores(1, nx);
+            commit(ke + nx);
+          } else {
+            commit(of + 1);
           }
         }
-        it += pc.n;
-        ++un;
+        if (!ok) break;
+        it += n;
       }
       if (!ok) {  // nothing may be in flight when TMEM is freed
-        umma::commit(drain);
+        commit(drain);
         umma::mbar_wait_bounded(drain, 0, kPcPolls);
       }
     }
   } else if (tid >= kPcLoad0) {
     // ----------------------------------------------------------- loaders
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcRegsLoad));
     const int lw = warp - kPcLoad0 / 32;
     constexpr int QC = D / 64;  // 64-byte column blocks of a row
     const int tr = lane & 7, cl = lane >> 3;
     const int lg = pool.lg_page, mask = pool.page() - 1;
     struct Tile { int b, h, tok0, lo, hi; bool any; };
     Tile cur, nxt;
-    int i = -1;
-    auto step = [&](Tile* t) {
-      if (i >= 0 && i + 1 < pc.n) ++i;
-      else if (pc.next()) i = 0;
-      else { t->any = false; return; }
-      t->any = true;
-      t->b = pc.b; t->h = pc.h; t->tok0 = (pc.tile + i) * kPcTok; t->lo = pc.lo; t->hi = pc.hi;
+    nxt.any = false;
+    int left = 0, un = 0;
+    bool ok = true;
+    auto step = [&](Tile* t) {  // the tile after *t
+      if (left > 0) {
+        --left;
+        t->tok0 += kPcTok;
+        return;
+      }
+      const int sl = un % kPcPieces;
+      ok = wait(nf + sl, (un / kPcPieces) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      t->any = false;
+      if (!ok) return;
+      const ChunkPiece& p = pieces[sl];
+      left = p.n - 1;
+      t->any = p.n > 0;
+      t->b = p.b; t->h = p.h; t->tok0 = p.tile * kPcTok; t->lo = p.lo; t->hi = p.hi;
+      umma::mbar_arrive(ne + sl);
+      ++un;
     };
     // lane l (mod 8) knows the page of the tile's l-th 16 tokens: -1 outside [lo, hi), -2 a bad id
     auto page_id = [&](const Tile& t) -> int {
@@ -254,19 +336,20 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) codes_to_f16<STORE>(w[e], &o[2 * e], &o[2 * e + 1]);
-          unsigned char* p = dst + tg * (16 * D) + (4 * c + cl) * 256 + tr * 16;
-          *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(p + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+          unsigned char* p = dst + c * kPcBlock + tg * 1024 + tr * 128;
+          *reinterpret_cast<uint4*>(p + 16 * ((2 * cl) ^ tr)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(p + 16 * ((2 * cl + 1) ^ tr)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
     };
-    step(&cur);
+    step(&nxt);
+    cur = nxt;
     int ids = page_id(cur);
     fetch(cur, ids, pool.k, kr);
     fetch(cur, ids, pool.v, vr);
-    bool ok = true;
     for (int it = 0; cur.any && ok; ++it) {
       step(&nxt);
+      if (!ok) break;
       const int ids_n = page_id(nxt);
       const int st = it % NS;
       float ks = 0.f, vs = 0.f;
@@ -301,21 +384,29 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     }
   } else {
     // ----------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPcRegsSoftmax));
     const int w = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t t_s = tmem + 128 * w + lanes, t_o = tmem + 256 + D * w + lanes;
     int it = 0, tc = 0, uc = 0;
     bool ok = true;
-    while (ok && pc.next()) {
-      const int R = pc.rt * kPcRows + 128 * w + r;
-      const bool two = pc.rows - pc.rt * kPcRows > 128, active = w == 0 || two;
+    for (int un = 0;; ++un) {
+      const int sl = un % kPcPieces;
+      ok = wait(nf + sl, (un / kPcPieces) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const ChunkPiece pc = pieces[sl];
+      umma::mbar_arrive(ne + sl);
+      if (pc.n == 0) break;
+      const int R = pc.row0 + 128 * w + r;
+      const bool two = pc.rows - pc.row0 > 128, active = w == 0 || two;
       const bool live = R < pc.rows;
+      const int Rl = live ? R : pc.rows - 1, tok_q = Rl / rq.G, head = pc.h * rq.G + Rl % rq.G;
       float cq = 0.f;
       if (active) {
         // ---- this thread's query row, scaled by a power of two, as f16
-        const int Rl = live ? R : pc.rows - 1;
-        const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)pc.b * a.q_sb) +
-                       (long)(pc.h * rq.G + Rl % rq.G) * a.q_sh + (long)(rq.q0(pc.b) + Rl / rq.G) * a.q_st;
+        const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)pc.b * a.q_sb) + (long)head * a.q_sh +
+                       (long)(pc.q0 + tok_q) * a.q_st;
         uint4 x[D / 8];
         float amax = 0.f;
 #pragma unroll
@@ -329,20 +420,26 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         e2 = e2 > 127 ? 0 : max(-100, min(100, e2));  // an infinite row keeps its values
         const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
         cq = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scaling;
-        unsigned char* dst = psm + L::q + w * L::tile + (r >> 3) * (16 * D) + (r & 7) * 16;
+        unsigned char* dst = psm + L::q + w * L::tile + (r >> 3) * 1024 + (r & 7) * 128;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
           const T* e = reinterpret_cast<const T*>(&x[c]);
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[k] = pack_f16(load_f(e + 2 * k) * down, load_f(e + 2 * k + 1) * down);
-          *reinterpret_cast<uint4*>(dst + 128 * c) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * kPcBlock + 16 * ((c & 7) ^ (r & 7))) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         umma::fence_proxy_async_smem();
       }
       umma::mbar_arrive(qf);
-      if (!active) { it += pc.n; if (pc.pieces(at.chunk)) begun = make_int4(pc.b, pc.h, pc.rt, pc.pieces(at.chunk)); continue; }
-      const int lim_lo = live ? pc.row_lo(R) : 0, lim_hi = live ? pc.row_hi(R) : 0;
+      if (!active) {
+        it += pc.n;
+        continue;
+      }
+      // the row sees [lim_lo, lim_hi)
+      const int last = pc.len - pc.q_len + tok_q;
+      const int lim_hi = live ? min(pc.len, last + 1) : 0;
+      const int lim_lo = !live ? 0 : rq.window > 0 ? max(pc.start, last - rq.window + 1) : pc.start;
       float m = -INFINITY, mv = -INFINITY, l = 0.f;
       for (int i = 0; i < pc.n; ++i) {
         const ChunkScales& sc = scales[(it + i) % L::ring];
@@ -357,30 +454,31 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
 #pragma unroll
         for (int g = 0; g < 8; ++g) bad |= sc.bad[g];
         const bool plain = __all_sync(0xffffffffu, e_lo <= 0 && e_hi >= kPcTok && !bad);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) umma::tmem_ld32(t_s + 32 * c, s[c]);
+        umma::tmem_wait_ld();
+        if (!plain) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int col = 32 * c + e;
+              if (col < e_lo || col >= e_hi || sc.bad[col >> 4]) s[c][e] = 0xff800000u;  // -inf
+            }
+        }
         // ---- the tile's maxima of x and of x + log2(vs)
         float tm = -INFINITY, tv = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          umma::tmem_ld32(t_s + 32 * c, s);
-          umma::tmem_wait_ld();
+        for (int g = 0; g < 8; ++g) {
+          const uint32_t* v = s[g >> 1] + 16 * (g & 1);
+          float bm = __uint_as_float(v[0]);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float bm = -INFINITY;
-            if (plain) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) bm = fmaxf(bm, __uint_as_float(s[16 * g + e]));
-            } else if (!sc.bad[2 * c + g]) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int col = 32 * c + 16 * g + e;
-                if (col >= e_lo && col < e_hi) bm = fmaxf(bm, __uint_as_float(s[16 * g + e]));
-              }
-            }
-            const float x = bm == -INFINITY ? -INFINITY : bm * (sc.ks[2 * c + g] * cq);
-            tm = fmaxf(tm, x);
-            tv = fmaxf(tv, x + sc.lv[2 * c + g]);
-          }
+          for (int e = 1; e < 15; e += 2) bm = fmaxf(fmaxf(bm, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+          bm = fmaxf(bm, __uint_as_float(v[15]));
+          const float x = bm * fmaxf(sc.ks[g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
+          tm = fmaxf(tm, x);
+          tv = fmaxf(tv, x + sc.lv[g]);
         }
         const bool grew = tm > m + 8.f || tv > mv + 8.f;
         if (__any_sync(0xffffffffu, grew)) {
@@ -390,14 +488,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           m = nm;
           mv = nv;
           if (i > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              umma::tmem_ld32(t_o + 32 * c, o);
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {  // few registers: S is held meanwhile
+              float o[16];
+              uint32_t u[16];
+              umma::tmem_ld16(t_o + 16 * c, o);
               umma::tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              umma::tmem_st32(t_o + 32 * c, o);
+              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+              umma::tmem_st16(t_o + 16 * c, u);
             }
             umma::tmem_wait_st();
           }
@@ -409,39 +508,21 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         const uint64_t base2 = pack2(base, base);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t s[32], p16[16];
-          umma::tmem_ld32(t_s + 32 * c, s);
-          umma::tmem_wait_ld();
+          uint32_t p16[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const float cg = sc.ks[2 * c + g] * cq, wg = fminf(sc.vs[2 * c + g] * fr, 0x1p100f);
-            if (plain) {
-              const uint64_t c2 = pack2(cg, cg), w2 = pack2(wg, wg);
+            const float cg = fmaxf(sc.ks[2 * c + g] * cq, 0x1p-126f), wg = fminf(sc.vs[2 * c + g] * fr, 0x1p100f);
+            const uint64_t c2 = pack2(cg, cg), w2 = pack2(wg, wg);
 #pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const uint64_t x2 = fma2(pack2(__uint_as_float(s[16 * g + e]), __uint_as_float(s[16 * g + e + 1])), c2, base2);
-                float x0, x1;
-                unpack2(x2, &x0, &x1);
-                const uint64_t p2 = pack2(exp2_fast(x0), exp2_fast(x1));
-                l2 = add2(l2, p2);
-                float y0, y1;
-                unpack2(mul2(p2, w2), &y0, &y1);
-                p16[8 * g + e / 2] = pack_f16(y0, y1);
-              }
-            } else {
-              const bool skip = sc.bad[2 * c + g];
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                float p[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int col = 32 * c + 16 * g + e + k;
-                  const bool see = !skip && col >= e_lo && col < e_hi;
-                  p[k] = see ? exp2_fast(fmaf(__uint_as_float(s[16 * g + e + k]), cg, base)) : 0.f;
-                  l += p[k];
-                }
-                p16[8 * g + e / 2] = pack_f16(p[0] * wg, p[1] * wg);
-              }
+            for (int e = 0; e < 16; e += 2) {
+              const uint64_t x2 = fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, base2);
+              float x0, x1;
+              unpack2(x2, &x0, &x1);
+              const uint64_t p2 = pack2(exp2_fast(x0), exp2_fast(x1));
+              l2 = add2(l2, p2);
+              float y0, y1;
+              unpack2(mul2(p2, w2), &y0, &y1);
+              p16[8 * g + e / 2] = pack_f16(y0, y1);
             }
           }
           umma::tmem_st16(t_s + 16 * c, p16);
@@ -461,12 +542,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       if (!ok) break;
       ++uc;
       umma::fence_after_sync();
-      const bool whole = pc.whole();
+      const bool whole = pc.whole;
       const float back = mv == -INFINITY ? 1.f : exp2_fast(mv - m);
       const float f = whole ? (l == 0.f ? 0.f : back / l) : back;
       const int row = 128 * w + r;
-      float* rec = a.part.rec + ((long)blockIdx.x * 2 + (pc.off == 0 ? 1 : 0)) * kPcRows * (D + 2);
-      const long orow = live ? (pc.out_row(R)) * a.out.Hq + pc.h * rq.G + R % rq.G : 0;
+      float* rec = a.part.rec + ((long)blockIdx.x * 2 + (pc.begins ? 1 : 0)) * kPcRows * (D + 2);
+      const long orow = ((rq.cu_q ? pc.q0 : (long)pc.b * rq.q_tokens) + tok_q) * a.out.Hq + head;
       T* dst = reinterpret_cast<T*>(a.out.out) + orow * D;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -500,9 +581,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           rec[kPcRows * D + kPcRows + row] = l;
         }
       }
-      if (pc.pieces(at.chunk)) begun = make_int4(pc.b, pc.h, pc.rt, pc.pieces(at.chunk));
     }
-    if (tid == 0) a.part.head[blockIdx.x] = ok ? begun : make_int4(0, 0, 0, 0);
   }
   umma::fence_before_sync();
   __syncthreads();

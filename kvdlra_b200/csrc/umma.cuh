@@ -30,6 +30,15 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t smem_addr, uint32_t lbo, 
   return d;
 }
 
+// The same with the 128-byte swizzle: rows of 128 bytes, eight of them to an
+// atom of 1024 (1024-byte aligned), whose 16-byte units are stored at unit
+// index ^ (row % 8).  K-major operand: `sbo` is the distance between groups of
+// eight rows; 128 bytes of K (lbo unused).  MN-major: a row is one k, `sbo` the
+// distance between groups of eight k, `lbo` between blocks of 128 bytes of N.
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+  return smem_desc(smem_addr, lbo, sbo) | ((uint64_t)2 << 61);
+}
+
 // Instruction descriptor of kind::tf32 with fp32 accumulation, both operands
 // K-major, dense: [4,6) D format (1 = F32), [7,10) A format (2 = TF32),
 // [10,13) B format (2 = TF32), [15] A major (0 = K), [16] B major (0 = K),
@@ -158,6 +167,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of a converged warp, the same one every time.  Products issued
+// under it from warp-uniform code keep their descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
 
 // Arrive on the mbarrier once every tcgen05.mma issued so far by this thread
 // has completed.
