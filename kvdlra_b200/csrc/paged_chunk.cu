@@ -1,11 +1,11 @@
 // Attention over 8-bit pages for requests of many query rows (chunks of a
 // prompt) on tcgen05 (sm_100a): bf16 and f16 queries, head_dim 64 and 128.
 //
-// One CTA of 13 warps per SM walks its run of the work list; a unit is
+// One CTA of 20 warps per SM walks its run of the work list; a unit is
 // (request, KV head, 256 query rows), a row (token, head of the group).  Per
 // 128-token tile:
-//   loaders (4 warps)  the page's codes from global memory, a tile ahead in
-//                      registers, converted exactly to f16 and written to shared
+//   loaders (4 warps for keys, 4 for values)  the page's codes from global
+//                      memory, a tile ahead in registers, converted exactly to f16 and written to shared
 //                      memory as rows of 64 dims with the 128-byte swizzle: the
 //                      same image is a K-major operand of the scores and an
 //                      MN-major one of the values.
@@ -36,12 +36,14 @@
 namespace kvd {
 
 constexpr int kPcRows = 256, kPcTok = 128;
-constexpr int kPcThreads = 512;            // 8 softmax warps, 4 loaders, issuer, planner (and 2 that wait)
-// registers per thread of the four warpgroups: a softmax thread holds its row
-// of S, a loader a tile's codes; their sum is what the CTA is launched with
-constexpr int kPcRegsSoftmax = 168, kPcRegsLoad = 128, kPcRegsIssue = 48;
-static_assert(2 * kPcRegsSoftmax + kPcRegsLoad + kPcRegsIssue == 4 * (65536 / kPcThreads), "register split");
-constexpr int kPcLoad0 = 256, kPcIssue0 = 384, kPcPlan0 = 416;
+constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, issuer, planner (and 2 that wait)
+// registers per thread of the five warpgroups: a softmax thread holds its row
+// of S, a loader its share of a tile's codes; their sum is what the CTA is
+// launched with (96 a thread)
+constexpr int kPcRegsLaunch = 65536 / kPcThreads / 8 * 8;
+constexpr int kPcRegsSoftmax = 160, kPcRegsLoad = 64, kPcRegsIssue = 32;
+static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
+constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
 constexpr long kPcPolls = 1L << 20;
 
@@ -57,9 +59,10 @@ struct ChunkArgs {
   PagedPart part;
 };
 
-struct ChunkScales {  // of one tile, per 16 tokens
-  float ks[8], vs[8], lv[8];  // lv = log2(vs)
-  int bad[8];                 // page id out of range
+struct alignas(16) ChunkScales {  // of one tile, per 16 tokens
+  float ks[8], lv[8];  // keys' scale, log2 of the values'
+  int bad;             // bit g: the g-th page id is out of range
+  int pad[3];
 };
 
 // A piece of the CTA's work, as the planner hands it to the other roles (their
@@ -71,17 +74,15 @@ struct ChunkPiece {
   int len, q_len, start, q0;
   int whole, begins;      // covers its unit; begins it
 };
-constexpr int kPcPieces = 4;  // pieces planned ahead
+constexpr int kPcPieces = 8;  // pieces planned ahead
 
 template <int D>
 struct ChunkSmem {
   static constexpr int NS = D == 64 ? 4 : 2;   // stages of keys, and of values
   static constexpr int tile = kPcTok * D * 2;  // f16 bytes of a 128-row operand
-  static constexpr int q = 0, v = q + 2 * tile, k = v + NS * tile, sc = k + NS * tile;
-  static constexpr int ring = 8;               // tiles whose scales are held: NS + 1 at least
-  static constexpr int bars = sc + ring * (int)sizeof(ChunkScales);
-  static constexpr int nbars = 4 * NS + 8 + 2 * kPcPieces;
-  static constexpr int total = bars + nbars * 8 + 1024;  // room to align
+  static constexpr int q = 0, v = q + 2 * tile, k = v + NS * tile;
+  static constexpr int total = k + NS * tile + 1024;  // room to align
+  static constexpr int ring = NS == 2 ? 4 : 8;        // tiles whose scales are held: NS + 1 at least
 };
 
 KVD_DEVICE uint64_t pack2(float a, float b) {
@@ -95,14 +96,15 @@ KVD_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-KVD_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 KVD_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+KVD_DEVICE float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -118,10 +120,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PagedPool& pool = a.pool;
   const PagedReqs& rq = a.reqs;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(psm + L::bars);
-  uint64_t *kf = bars, *ke = kf + NS, *vf = ke + NS, *ve = vf + NS, *sf = ve + NS, *pf = sf + 2, *of = pf + 2, *qf = of + 2, *drain = qf + 1,
-           *nf = drain + 1, *ne = nf + kPcPieces;
-  ChunkScales* scales = reinterpret_cast<ChunkScales*>(psm + L::sc);
+  __shared__ ChunkScales scales[L::ring];
+  __shared__ uint64_t kf[NS], ke[NS], vf[NS], ve[NS];  // a stage of keys, of values: full, empty
+  __shared__ uint64_t sf[2], pf[2], of[2], qf, drain;  // scores, weights, outputs of a row tile; queries
+  __shared__ uint64_t nf[kPcPieces], ne[kPcPieces];    // pieces
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
     umma::tmem_alloc(&tmem_base, 512);
@@ -142,10 +144,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     }
     for (int i = 0; i < kPcPieces; ++i) {
       umma::mbar_init(nf + i, 1);
-      umma::mbar_init(ne + i, 256 + 128 + 1);
+      umma::mbar_init(ne + i, 256 + 256 + 1);
     }
-    umma::mbar_init(qf, 256);
-    umma::mbar_init(drain, 1);
+    umma::mbar_init(&qf, 256);
+    umma::mbar_init(&drain, 1);
     umma::mbar_fence_init();
   }
   umma::fence_before_sync();
@@ -195,8 +197,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       auto scores = [&](int w, int stage) {
         const uint64_t q_w = q_d + w * (L::tile >> 4), k_s = k_d + stage * (L::tile >> 4);
         if (umma::elect_one()) {
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
+#pragma unroll 1
+          for (int j = 0; j < D / 16; ++j) {  // unrolled, the descriptors of all stages would fill the registers
             const uint64_t at_j = ((j >> 2) * kPcBlock + 32 * (j & 3)) >> 4;
             umma::mma_bf16(tmem + 128 * w, q_w + at_j, k_s + at_j, id_s, j > 0);
           }
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       auto values = [&](int w, int stage, bool acc) {
         const uint64_t v_s = v_d + stage * (L::tile >> 4);
         if (umma::elect_one()) {
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < kPcTok / 16; ++j)
             umma::mma_f16_ts(tmem + 256 + D * w, tmem + 128 * w + 8 * j, v_s + ((2048 * j) >> 4), id_o, acc || j > 0);
         }
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         const bool two = __shfl_sync(0xffffffffu, pieces[sl].rows - pieces[sl].row0 > 128, 0);
         if (lane == 0) umma::mbar_arrive(ne + sl);
         if (n == 0) break;
-        ok = wait_all(qf, un & 1) && wait_all(kf + it % NS, (it / NS) & 1);
+        ok = wait_all(&qf, un & 1) && wait_all(kf + it % NS, (it / NS) & 1);
         if (!ok) break;
         umma::fence_after_sync();
         scores(0, it % NS);
@@ -268,20 +270,27 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         it += n;
       }
       if (!ok) {  // nothing may be in flight when TMEM is freed
-        commit(drain);
-        umma::mbar_wait_bounded(drain, 0, kPcPolls);
+        commit(&drain);
+        umma::mbar_wait_bounded(&drain, 0, kPcPolls);
       }
     }
   } else if (tid >= kPcLoad0) {
     // ----------------------------------------------------------- loaders
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcRegsLoad));
-    const int lw = warp - kPcLoad0 / 32;
+    // keys by the first warpgroup, values by the second
+    const bool keys = warp < kPcLoad0 / 32 + 4;
+    const int lw = (warp - kPcLoad0 / 32) & 3;
+    const unsigned char* codes = keys ? pool.k : pool.v;
+    unsigned char* stages = psm + (keys ? L::k : L::v);
+    uint64_t *full = keys ? kf : vf, *empty = keys ? ke : ve;
     constexpr int QC = D / 64;  // 64-byte column blocks of a row
     const int tr = lane & 7, cl = lane >> 3;
     const int lg = pool.lg_page, mask = pool.page() - 1;
-    struct Tile { int b, h, tok0, lo, hi; bool any; };
-    Tile cur, nxt;
-    nxt.any = false;
+    // A tile is a piece's slot and a token; the piece stays in its slot until the
+    // tile after it is current.  Three are under way: the current one (converted),
+    // the next (codes and scales on their way) and the one after (page ids).
+    struct Tile { int sl, tok0; };  // sl < 0: none
+    Tile cur, nxt, aft = {0, 0};
     int left = 0, un = 0;
     bool ok = true;
     auto step = [&](Tile* t) {  // the tile after *t
@@ -290,49 +299,54 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         t->tok0 += kPcTok;
         return;
       }
+      if (t->sl < 0) return;
       const int sl = un % kPcPieces;
       ok = wait(nf + sl, (un / kPcPieces) & 1);
       ok = __all_sync(0xffffffffu, ok);
-      t->any = false;
-      if (!ok) return;
-      const ChunkPiece& p = pieces[sl];
-      left = p.n - 1;
-      t->any = p.n > 0;
-      t->b = p.b; t->h = p.h; t->tok0 = p.tile * kPcTok; t->lo = p.lo; t->hi = p.hi;
-      umma::mbar_arrive(ne + sl);
+      const int n = ok ? pieces[sl].n : 0;
+      if (n == 0) {
+        t->sl = -1;
+        return;
+      }
+      left = n - 1;
+      t->sl = sl;
+      t->tok0 = pieces[sl].tile * kPcTok;
       ++un;
     };
     // lane l (mod 8) knows the page of the tile's l-th 16 tokens: -1 outside [lo, hi), -2 a bad id
     auto page_id = [&](const Tile& t) -> int {
+      if (t.sl < 0) return -1;
+      const ChunkPiece& p = pieces[t.sl];
       const int tok = t.tok0 + 16 * tr;
-      if (!t.any || tok >= t.hi || tok + 16 <= t.lo) return -1;
-      const int id = a.table[(long)t.b * a.table_stride + (tok >> lg)];
+      if (tok >= p.hi || tok + 16 <= p.lo) return -1;
+      const int id = a.table[(long)p.b * a.table_stride + (tok >> lg)];
       return id < 0 || id >= pool.num_pages ? -2 : id;
     };
-    uint4 kr[4][QC], vr[4][QC];
-    auto fetch = [&](const Tile& t, int ids, const unsigned char* codes, uint4 (&r)[4][QC]) {
+    uint4 raw[4][QC];
+    auto fetch = [&](const Tile& t, int ids) {
+      const int sl = max(0, t.sl), lo = pieces[sl].lo, hi = t.sl < 0 ? 0 : pieces[sl].hi;
+      const unsigned char* base = codes + (long)pieces[sl].h * pool.head_stride + 16 * cl;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int tg = 4 * k + lw, tok = t.tok0 + 8 * tg + tr;
         const int id = __shfl_sync(0xffffffffu, ids, tg >> 1);
-        const bool live = t.any && id >= 0 && tok >= t.lo && tok < t.hi;
-        const unsigned char* p = codes + (long)id * pool.page_stride + (long)t.h * pool.head_stride +
-                                 (long)(tok & mask) * pool.slot_stride + 16 * cl;
+        const bool live = id >= 0 && tok >= lo && tok < hi;
+        const unsigned char* p = base + (long)id * pool.page_stride + (long)(tok & mask) * pool.slot_stride;
 #pragma unroll
         for (int c = 0; c < QC; ++c) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (live) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p + 64 * c));
-          r[k][c] = x;
+          raw[k][c] = x;
         }
       }
     };
-    auto put = [&](unsigned char* dst, const uint4 (&r)[4][QC]) {
+    auto put = [&](unsigned char* dst) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int tg = 4 * k + lw;
 #pragma unroll
         for (int c = 0; c < QC; ++c) {
-          const uint32_t w[4] = {r[k][c].x, r[k][c].y, r[k][c].z, r[k][c].w};
+          const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) codes_to_f16<STORE>(w[e], &o[2 * e], &o[2 * e + 1]);
@@ -342,45 +356,51 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         }
       }
     };
-    step(&nxt);
-    cur = nxt;
-    int ids = page_id(cur);
-    fetch(cur, ids, pool.k, kr);
-    fetch(cur, ids, pool.v, vr);
-    for (int it = 0; cur.any && ok; ++it) {
-      step(&nxt);
-      if (!ok) break;
-      const int ids_n = page_id(nxt);
-      const int st = it % NS;
-      float ks = 0.f, vs = 0.f;
-      if (lw == 0 && lane < 8 && ids >= 0) {
-        ks = pool.ks[(long)ids * pool.scale_stride + cur.h];
-        vs = pool.vs[(long)ids * pool.scale_stride + cur.h];
+    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
+    auto scale = [&](const Tile& t, int ids, float* k, float* v) {
+      *k = *v = 0.f;
+      if (keys && lw == 0 && lane < 8 && ids >= 0) {
+        const long at_s = (long)ids * pool.scale_stride + pieces[t.sl].h;
+        *k = pool.ks[at_s];
+        *v = pool.vs[at_s];
       }
-      ok = wait(ke + st, ((it / NS) & 1) ^ 1);
+    };
+    step(&aft);
+    cur = aft;
+    int ids = page_id(cur);
+    step(&aft);
+    nxt = aft;
+    int ids_n = page_id(nxt);
+    fetch(cur, ids);
+    scale(cur, ids, &ks, &vs);
+    for (int it = 0; cur.sl >= 0 && ok; ++it) {
+      step(&aft);
+      if (!ok) break;
+      const int ids_a = page_id(aft);
+      scale(nxt, ids_n, &ks_n, &vs_n);
+      const int st = it % NS;
+      ok = wait(empty + st, ((it / NS) & 1) ^ 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      put(psm + L::k + st * L::tile, kr);
-      if (lw == 0 && lane < 8) {
+      put(stages + st * L::tile);
+      if (keys && lw == 0 && lane < 8) {
         ChunkScales& s = scales[it % L::ring];
         s.ks[lane] = ks;
-        s.vs[lane] = vs;
         s.lv[lane] = log2f(vs);
-        s.bad[lane] = ids == -2;
+        const uint32_t bad = __ballot_sync(0xffu, ids == -2);
+        if (lane == 0) s.bad = (int)bad;
         if (ids == -2) pool.flag(kStatusBounds, kPagedBadPage);
       }
       umma::fence_proxy_async_smem();
-      umma::mbar_arrive(kf + st);
-      fetch(nxt, ids_n, pool.k, kr);
-      ok = wait(ve + st, ((it / NS) & 1) ^ 1);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      put(psm + L::v + st * L::tile, vr);
-      umma::fence_proxy_async_smem();
-      umma::mbar_arrive(vf + st);
-      fetch(nxt, ids_n, pool.v, vr);
+      umma::mbar_arrive(full + st);
+      fetch(nxt, ids_n);
+      if (nxt.sl != cur.sl) umma::mbar_arrive(ne + cur.sl);
       cur = nxt;
+      nxt = aft;
       ids = ids_n;
+      ids_n = ids_a;
+      ks = ks_n;
+      vs = vs_n;
     }
   } else {
     // ----------------------------------------------------------- softmax
@@ -395,15 +415,19 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       ok = wait(nf + sl, (un / kPcPieces) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const ChunkPiece pc = pieces[sl];
-      umma::mbar_arrive(ne + sl);
-      if (pc.n == 0) break;
-      const int R = pc.row0 + 128 * w + r;
-      const bool two = pc.rows - pc.row0 > 128, active = w == 0 || two;
-      const bool live = R < pc.rows;
-      const int Rl = live ? R : pc.rows - 1, tok_q = Rl / rq.G, head = pc.h * rq.G + Rl % rq.G;
+      const ChunkPiece& pc = pieces[sl];  // stays until this thread has written the result
+      const int n = pc.n;
+      if (n == 0) break;
+      const bool active = w == 0 || pc.rows - pc.row0 > 128;
       float cq = 0.f;
+      int lim_lo = 0, lim_hi = 0;  // the row sees [lim_lo, lim_hi)
       if (active) {
+        const int R = min(pc.rows - 1, pc.row0 + 128 * w + r), tok_q = R / rq.G, head = pc.h * rq.G + R % rq.G;
+        if (pc.row0 + 128 * w + r < pc.rows) {
+          const int last = pc.len - pc.q_len + tok_q;
+          lim_hi = min(pc.len, last + 1);
+          lim_lo = rq.window > 0 ? max(pc.start, last - rq.window + 1) : pc.start;
+        }
         // ---- this thread's query row, scaled by a power of two, as f16
         const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)pc.b * a.q_sb) + (long)head * a.q_sh +
                        (long)(pc.q0 + tok_q) * a.q_st;
@@ -431,17 +455,14 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         }
         umma::fence_proxy_async_smem();
       }
-      umma::mbar_arrive(qf);
+      umma::mbar_arrive(&qf);
       if (!active) {
-        it += pc.n;
+        umma::mbar_arrive(ne + sl);
+        it += n;
         continue;
       }
-      // the row sees [lim_lo, lim_hi)
-      const int last = pc.len - pc.q_len + tok_q;
-      const int lim_hi = live ? min(pc.len, last + 1) : 0;
-      const int lim_lo = !live ? 0 : rq.window > 0 ? max(pc.start, last - rq.window + 1) : pc.start;
       float m = -INFINITY, mv = -INFINITY, l = 0.f;
-      for (int i = 0; i < pc.n; ++i) {
+      for (int i = 0; i < n; ++i) {
         const ChunkScales& sc = scales[(it + i) % L::ring];
         ok = wait(sf + w, tc & 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -450,33 +471,37 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         umma::fence_after_sync();
         const int tok0 = (pc.tile + i) * kPcTok;
         const int e_lo = lim_lo - tok0, e_hi = lim_hi - tok0;  // visible columns
-        int bad = 0;
-#pragma unroll
-        for (int g = 0; g < 8; ++g) bad |= sc.bad[g];
+        const int bad = sc.bad;
         const bool plain = __all_sync(0xffffffffu, e_lo <= 0 && e_hi >= kPcTok && !bad);
+        // ---- the tile's maxima of x and of x + log2(vs).  Reads of TMEM are slow
+        // while the tensor core works for the other row tile: one wait for all of S.
+        // Its last quarter is read again later, to free registers in between.
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) umma::tmem_ld32(t_s + 32 * c, s[c]);
         umma::tmem_wait_ld();
-        if (!plain) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
+        auto hide = [&](int c) {
+          if (!plain) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const int col = 32 * c + e;
-              if (col < e_lo || col >= e_hi || sc.bad[col >> 4]) s[c][e] = 0xff800000u;  // -inf
+              if (col < e_lo || col >= e_hi || (bad >> (col >> 4) & 1)) s[c][e] = 0xff800000u;  // -inf
             }
-        }
-        // ---- the tile's maxima of x and of x + log2(vs)
+          }
+        };
         float tm = -INFINITY, tv = -INFINITY;
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
+          if (g % 2 == 0) hide(g / 2);
           const uint32_t* v = s[g >> 1] + 16 * (g & 1);
-          float bm = __uint_as_float(v[0]);
+          float b0 = __uint_as_float(v[0]), b1 = __uint_as_float(v[1]);
 #pragma unroll
-          for (int e = 1; e < 15; e += 2) bm = fmaxf(fmaxf(bm, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
-          bm = fmaxf(bm, __uint_as_float(v[15]));
-          const float x = bm * fmaxf(sc.ks[g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
+          for (int e = 2; e < 14; e += 4) {
+            b0 = max3(b0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            b1 = max3(b1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+          }
+          b0 = max3(b0, __uint_as_float(v[14]), __uint_as_float(v[15]));
+          const float x = fmaxf(b0, b1) * fmaxf(sc.ks[g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
           tm = fmaxf(tm, x);
           tv = fmaxf(tv, x + sc.lv[g]);
         }
@@ -489,52 +514,56 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           mv = nv;
           if (i > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {  // few registers: S is held meanwhile
-              float o[16];
-              uint32_t u[16];
-              umma::tmem_ld16(t_o + 16 * c, o);
+            for (int c = 0; c < D / 8; ++c) {  // few registers: S is held meanwhile
+              uint32_t u[8];
+              umma::tmem_ld8(t_o + 8 * c, u);
               umma::tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
-              umma::tmem_st16(t_o + 16 * c, u);
+              for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+              umma::tmem_st8(t_o + 8 * c, u);
             }
             umma::tmem_wait_st();
           }
         }
-        // ---- weights
+        // ---- weights: p vs 2^(m - mv) = 2^(x - m + d), d = log2(vs) + m - mv, d >= -100
+        // (a smaller scale's values are nothing beside the row's largest); their sum
+        // over a page's tokens, times 2^-d, goes to l
         const float base = m == -INFINITY ? 0.f : -m;
-        const float fr = mv == -INFINITY ? 0.f : exp2_fast(m - mv);
-        uint64_t l2 = pack2(0.f, 0.f);
-        const uint64_t base2 = pack2(base, base);
+        const float dm = mv == -INFINITY ? 0.f : m - mv;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          if (c == 1) umma::tmem_ld32(t_s + 96, s[3]);  // P stays below column 64
+          if (c == 3) {
+            umma::tmem_wait_ld();
+            hide(3);
+          }
           uint32_t p16[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const float cg = fmaxf(sc.ks[2 * c + g] * cq, 0x1p-126f), wg = fminf(sc.vs[2 * c + g] * fr, 0x1p100f);
-            const uint64_t c2 = pack2(cg, cg), w2 = pack2(wg, wg);
+            const float cg = fmaxf(sc.ks[2 * c + g] * cq, 0x1p-126f);
+            const float d = fmaxf(sc.lv[2 * c + g] + dm, -100.f), bg = base + d;
+            const uint64_t c2 = pack2(cg, cg), b2 = pack2(bg, bg);
+            uint64_t l2 = pack2(0.f, 0.f);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const uint64_t x2 = fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, base2);
               float x0, x1;
-              unpack2(x2, &x0, &x1);
-              const uint64_t p2 = pack2(exp2_fast(x0), exp2_fast(x1));
-              l2 = add2(l2, p2);
-              float y0, y1;
-              unpack2(mul2(p2, w2), &y0, &y1);
-              p16[8 * g + e / 2] = pack_f16(y0, y1);
+              unpack2(fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, b2), &x0, &x1);
+              x0 = exp2_fast(x0);
+              x1 = exp2_fast(x1);
+              l2 = add2(l2, pack2(x0, x1));
+              p16[8 * g + e / 2] = pack_f16(x0, x1);
             }
+            float l0, l1;
+            unpack2(l2, &l0, &l1);
+            l = fmaf(l0 + l1, exp2_fast(-d), l);
           }
           umma::tmem_st16(t_s + 16 * c, p16);
         }
-        float l0, l1;
-        unpack2(l2, &l0, &l1);
-        l += l0 + l1;
         umma::tmem_wait_st();
         umma::fence_before_sync();
         umma::mbar_arrive(pf + w);
       }
-      it += pc.n;
+      it += n;
       if (!ok) break;
       // ---- the row's result, or this CTA's record of it
       ok = wait(of + w, uc & 1);
@@ -542,7 +571,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       if (!ok) break;
       ++uc;
       umma::fence_after_sync();
-      const bool whole = pc.whole;
+      const int R = pc.row0 + 128 * w + r, tok_q = R / rq.G, head = pc.h * rq.G + R % rq.G;
+      const bool whole = pc.whole, live = R < pc.rows;
       const float back = mv == -INFINITY ? 1.f : exp2_fast(mv - m);
       const float f = whole ? (l == 0.f ? 0.f : back / l) : back;
       const int row = 128 * w + r;
@@ -581,6 +611,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           rec[kPcRows * D + kPcRows + row] = l;
         }
       }
+      umma::mbar_arrive(ne + sl);
     }
   }
   umma::fence_before_sync();
