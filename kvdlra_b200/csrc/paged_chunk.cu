@@ -41,7 +41,7 @@ constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, issuer
 // of S, a loader its share of a tile's codes; their sum is what the CTA is
 // launched with (96 a thread)
 constexpr int kPcRegsLaunch = 65536 / kPcThreads / 8 * 8;
-constexpr int kPcRegsSoftmax = 160, kPcRegsLoad = 64, kPcRegsIssue = 32;
+constexpr int kPcRegsSoftmax = 152, kPcRegsLoad = 64, kPcRegsIssue = 48;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
 constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;  // a wait gave up
   __shared__ ChunkPiece pieces[kPcPieces];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be warp-uniform
   const PagedPool& pool = a.pool;
   const PagedReqs& rq = a.reqs;
   __shared__ ChunkScales scales[L::ring];
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     return false;
   };
 
-  if (tid >= kPcIssue0) {
+  if (warp >= kPcIssue0 / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcRegsIssue));
     if (warp == kPcPlan0 / 32 && lane == 0) {
       // ---------------------------------------------------------- planner
@@ -189,29 +190,29 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     } else if (warp == kPcIssue0 / 32) {
       // ----------------------------------------------------------- issuer
       // the whole warp walks, one lane issues: descriptors stay in uniform registers
-      const uint64_t q_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::q), 16, 1024);
       const uint64_t k_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::k), 16, 1024);
-      const uint64_t v_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::v), kPcBlock, 1024);
+      const uint32_t hi = (uint32_t)(k_d >> 32), k_lo = (uint32_t)k_d;
+      const uint32_t q_lo = k_lo - ((L::k - L::q) >> 4);  // an address counts 16 bytes
+      const uint32_t v_lo = (uint32_t)umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::v), kPcBlock, 1024);
       constexpr uint32_t id_s = umma::idesc_f16(128, kPcTok, false), id_o = umma::idesc_f16(128, D, true);
-      // a descriptor's address field counts 16 bytes
       auto scores = [&](int w, int stage) {
-        const uint64_t q_w = q_d + w * (L::tile >> 4), k_s = k_d + stage * (L::tile >> 4);
+        const uint32_t q_w = q_lo + w * (L::tile >> 4), k_s = k_lo + stage * (L::tile >> 4);
         if (umma::elect_one()) {
-#pragma unroll 1
-          for (int j = 0; j < D / 16; ++j) {  // unrolled, the descriptors of all stages would fill the registers
-            const uint64_t at_j = ((j >> 2) * kPcBlock + 32 * (j & 3)) >> 4;
-            umma::mma_bf16(tmem + 128 * w, q_w + at_j, k_s + at_j, id_s, j > 0);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            const uint32_t at_j = ((j >> 2) * kPcBlock + 32 * (j & 3)) >> 4;
+            umma::mma_f16_ss_lo(tmem + 128 * w, q_w + at_j, k_s + at_j, hi, id_s, j > 0);
           }
           umma::commit(sf + w);
         }
         __syncwarp();
       };
       auto values = [&](int w, int stage, bool acc) {
-        const uint64_t v_s = v_d + stage * (L::tile >> 4);
+        const uint32_t v_s = v_lo + stage * (L::tile >> 4);
         if (umma::elect_one()) {
-#pragma unroll 1
+#pragma unroll
           for (int j = 0; j < kPcTok / 16; ++j)
-            umma::mma_f16_ts(tmem + 256 + D * w, tmem + 128 * w + 8 * j, v_s + ((2048 * j) >> 4), id_o, acc || j > 0);
+            umma::mma_f16_ts_lo(tmem + 256 + D * w, tmem + 128 * w + 8 * j, v_s + ((2048 * j) >> 4), hi, id_o, acc || j > 0);
         }
         __syncwarp();
       };
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         umma::mbar_wait_bounded(&drain, 0, kPcPolls);
       }
     }
-  } else if (tid >= kPcLoad0) {
+  } else if (warp >= kPcLoad0 / 32) {
     // ----------------------------------------------------------- loaders
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcRegsLoad));
     // keys by the first warpgroup, values by the second
@@ -284,7 +285,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     unsigned char* stages = psm + (keys ? L::k : L::v);
     uint64_t *full = keys ? kf : vf, *empty = keys ? ke : ve;
     constexpr int QC = D / 64;  // 64-byte column blocks of a row
-    const int tr = lane & 7, cl = lane >> 3;
+    // A lane's token of eight, and its 16 bytes of a 64-byte block.  At head_dim
+    // 128 odd tokens take the blocks in the other order: the eight lanes of a
+    // memory cycle then touch every bank once, in the load and in the store.
+    const int tr = lane >> 2, cl = lane & 3;
     const int lg = pool.lg_page, mask = pool.page() - 1;
     // A tile is a piece's slot and a token; the piece stays in its slot until the
     // tile after it is current.  Three are under way: the current one (converted),
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     auto page_id = [&](const Tile& t) -> int {
       if (t.sl < 0) return -1;
       const ChunkPiece& p = pieces[t.sl];
-      const int tok = t.tok0 + 16 * tr;
+      const int tok = t.tok0 + 16 * (lane & 7);
       if (tok >= p.hi || tok + 16 <= p.lo) return -1;
       const int id = a.table[(long)p.b * a.table_stride + (tok >> lg)];
       return id < 0 || id >= pool.num_pages ? -2 : id;
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < QC; ++c) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (live) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p + 64 * c));
+          if (live) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p + 64 * (c ^ (QC - 1 & tr))));
           raw[k][c] = x;
         }
       }
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) codes_to_f16<STORE>(w[e], &o[2 * e], &o[2 * e + 1]);
-          unsigned char* p = dst + c * kPcBlock + tg * 1024 + tr * 128;
+          unsigned char* p = dst + (c ^ (QC - 1 & tr)) * kPcBlock + tg * 1024 + tr * 128;
           *reinterpret_cast<uint4*>(p + 16 * ((2 * cl) ^ tr)) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(p + 16 * ((2 * cl + 1) ^ tr)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
