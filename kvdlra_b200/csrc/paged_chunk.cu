@@ -30,18 +30,21 @@
 // Bound, per tile of 256 rows x 128 tokens at head_dim 128 and clock: tensor
 // core 2048, exponentials 2048 (16 a clock), shared memory about 2048 (Q, K and
 // V operands, and the converted tiles).
+#include <type_traits>
+
 #include "paged.cuh"
 #include "umma.cuh"
 
 namespace kvd {
 
-constexpr int kPcRows = 256, kPcTok = 128;
+constexpr int kPcRows = 256, kPcTok = 128;  // rows of a unit, tokens of a tile
+constexpr int kPcSub = 64;                  // tokens of a subtile: S has two buffers of them
 constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, issuer, planner (and 2 that wait)
 // registers per thread of the five warpgroups: a softmax thread holds its row
 // of S, a loader its share of a tile's codes; their sum is what the CTA is
 // launched with (96 a thread)
 constexpr int kPcRegsLaunch = 65536 / kPcThreads / 8 * 8;
-constexpr int kPcRegsSoftmax = 152, kPcRegsLoad = 64, kPcRegsIssue = 48;
+constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
 constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
@@ -123,7 +126,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   const PagedReqs& rq = a.reqs;
   __shared__ ChunkScales scales[L::ring];
   __shared__ uint64_t kf[NS], ke[NS], vf[NS], ve[NS];  // a stage of keys, of values: full, empty
-  __shared__ uint64_t sf[2], pf[2], of[2], qf, drain;  // scores, weights, outputs of a row tile; queries
+  __shared__ uint64_t sf[2][2], pf[2][2];              // scores, weights of (row tile, S buffer)
+  __shared__ uint64_t of[2], qf, drain;                // a subtile's product into O of a row tile; queries
   __shared__ uint64_t nf[kPcPieces], ne[kPcPieces];    // pieces
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
@@ -139,8 +143,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       umma::mbar_init(ve + i, 1);
     }
     for (int w = 0; w < 2; ++w) {
-      umma::mbar_init(sf + w, 1);
-      umma::mbar_init(pf + w, 128);
+      for (int b = 0; b < 2; ++b) {
+        umma::mbar_init(&sf[w][b], 1);
+        umma::mbar_init(&pf[w][b], 128);
+      }
       umma::mbar_init(of + w, 1);
     }
     for (int i = 0; i < kPcPieces; ++i) {
@@ -194,25 +200,27 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       const uint32_t hi = (uint32_t)(k_d >> 32), k_lo = (uint32_t)k_d;
       const uint32_t q_lo = k_lo - ((L::k - L::q) >> 4);  // an address counts 16 bytes
       const uint32_t v_lo = (uint32_t)umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::v), kPcBlock, 1024);
-      constexpr uint32_t id_s = umma::idesc_f16(128, kPcTok, false), id_o = umma::idesc_f16(128, D, true);
-      auto scores = [&](int w, int stage) {
-        const uint32_t q_w = q_lo + w * (L::tile >> 4), k_s = k_lo + stage * (L::tile >> 4);
+      constexpr uint32_t id_s = umma::idesc_f16(128, kPcSub, false), id_o = umma::idesc_f16(128, D, true);
+      // subtile b of a stage, S buffer b
+      auto scores = [&](int w, int stage, int b) {
+        const uint32_t q_w = q_lo + w * (L::tile >> 4), k_s = k_lo + stage * (L::tile >> 4) + b * (kPcSub * 128 >> 4);
         if (umma::elect_one()) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             const uint32_t at_j = ((j >> 2) * kPcBlock + 32 * (j & 3)) >> 4;
-            umma::mma_f16_ss_lo(tmem + 128 * w, q_w + at_j, k_s + at_j, hi, id_s, j > 0);
+            umma::mma_f16_ss_lo(tmem + 128 * w + 64 * b, q_w + at_j, k_s + at_j, hi, id_s, j > 0);
           }
-          umma::commit(sf + w);
+          umma::commit(&sf[w][b]);
         }
         __syncwarp();
       };
-      auto values = [&](int w, int stage, bool acc) {
-        const uint32_t v_s = v_lo + stage * (L::tile >> 4);
+      auto values = [&](int w, int stage, int b, bool acc) {
+        const uint32_t v_s = v_lo + stage * (L::tile >> 4) + b * (kPcSub * 128 >> 4);
         if (umma::elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kPcTok / 16; ++j)
-            umma::mma_f16_ts_lo(tmem + 256 + D * w, tmem + 128 * w + 8 * j, v_s + ((2048 * j) >> 4), hi, id_o, acc || j > 0);
+          for (int j = 0; j < kPcSub / 16; ++j)
+            umma::mma_f16_ts_lo(tmem + 256 + D * w, tmem + 128 * w + 64 * b + 8 * j, v_s + ((2048 * j) >> 4), hi, id_o, acc || j > 0);
+          umma::commit(&of[w]);
         }
         __syncwarp();
       };
@@ -221,7 +229,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         __syncwarp();
       };
       auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-      int it = 0, tc0 = 0, tc1 = 0;
+      int it = 0, t0 = 0, t1 = 0;  // tiles so far, of all units and by row tile
       bool ok = true;
       for (int un = 0;; ++un) {
         const int sl = un % kPcPieces;
@@ -234,38 +242,41 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         ok = wait_all(&qf, un & 1) && wait_all(kf + it % NS, (it / NS) & 1);
         if (!ok) break;
         umma::fence_after_sync();
-        scores(0, it % NS);
-        if (two) scores(1, it % NS);
+        for (int b = 0; b < 2; ++b) {
+          scores(0, it % NS, b);
+          if (two) scores(1, it % NS, b);
+        }
         commit(ke + it % NS);
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < n && ok; ++i) {
           const int g = it + i, st = g % NS, nx = (g + 1) % NS;
           const bool more = i + 1 < n;
-          ok = wait_all(vf + st, (g / NS) & 1) && wait_all(pf, tc0++ & 1);
-          if (!ok) break;
-          umma::fence_after_sync();
-          values(0, st, i > 0);
-          if (!two) commit(ve + st);
-          if (more) {
-            ok = wait_all(kf + nx, ((g + 1) / NS) & 1);
+          ok = wait_all(vf + st, (g / NS) & 1);
+          for (int b = 0; b < 2 && ok; ++b) {
+            // O += P V of this subtile, then S of the next tile's over its P: the
+            // tensor core takes one thread's products in order
+            ok = wait_all(&pf[0][b], t0 & 1);
             if (!ok) break;
             umma::fence_after_sync();
-            scores(0, nx);  // S over P: the tensor core takes one thread's products in order
-            if (!two) commit(ke + nx);
-          } else {
-            commit(of);
+            values(0, st, b, i > 0 || b > 0);
+            if (b == 0 && more) {
+              ok = wait_all(kf + nx, ((g + 1) / NS) & 1);
+              if (!ok) break;
+              umma::fence_after_sync();
+            }
+            if (more) scores(0, nx, b);
+            if (two) {
+              ok = wait_all(&pf[1][b], t1 & 1);
+              if (!ok) break;
+              umma::fence_after_sync();
+              values(1, st, b, i > 0 || b > 0);
+              if (more) scores(1, nx, b);
+            }
           }
-          if (!two) continue;
-          ok = wait_all(pf + 1, tc1++ & 1);
           if (!ok) break;
-          umma::fence_after_sync();
-          values(1, st, i > 0);
+          ++t0;
+          if (two) ++t1;
           commit(ve + st);
-          if (more) {
-            scores(1, nx);
-            commit(ke + nx);
-          } else {
-            commit(of + 1);
-          }
+          if (more) commit(ke + nx);
         }
         if (!ok) break;
         it += n;
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     const int w = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t t_s = tmem + 128 * w + lanes, t_o = tmem + 256 + D * w + lanes;
-    int it = 0, tc = 0, uc = 0;
+    int it = 0, tc = 0;
     bool ok = true;
     for (int un = 0;; ++un) {
       const int sl = un % kPcPieces;
@@ -435,12 +446,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         // ---- this thread's query row, scaled by a power of two, as f16
         const T* src = reinterpret_cast<const T*>(a.q) + (rq.cu_q ? 0 : (long)pc.b * a.q_sb) + (long)head * a.q_sh +
                        (long)(pc.q0 + tok_q) * a.q_st;
-        uint4 x[D / 8];
         float amax = 0.f;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
-          x[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-          const T* e = reinterpret_cast<const T*>(&x[c]);
+          const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * c);
+          const T* e = reinterpret_cast<const T*>(&x);
 #pragma unroll
           for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(load_f(e + k)));
         }
@@ -449,9 +459,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
         cq = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scaling;
         unsigned char* dst = psm + L::q + w * L::tile + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
-          const T* e = reinterpret_cast<const T*>(&x[c]);
+          const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * c);
+          const T* e = reinterpret_cast<const T*>(&x);
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[k] = pack_f16(load_f(e + 2 * k) * down, load_f(e + 2 * k + 1) * down);
@@ -466,114 +477,117 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         continue;
       }
       float m = -INFINITY, mv = -INFINITY, l = 0.f;
-      for (int i = 0; i < n; ++i) {
-        const ChunkScales& sc = scales[(it + i) % L::ring];
-        ok = wait(sf + w, tc & 1);
+      for (int u = 0; u < 2 * n; ++u) {  // subtiles
+        const ChunkScales& sc = scales[(it + (u >> 1)) % L::ring];
+        const int b = u & 1, g0 = 4 * b;
+        ok = wait(&sf[w][b], (tc + (u >> 1)) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++tc;
         umma::fence_after_sync();
-        const int tok0 = (pc.tile + i) * kPcTok;
+        const uint32_t t_b = t_s + 64 * b;
+        const int tok0 = pc.tile * kPcTok + u * kPcSub;
         const int e_lo = lim_lo - tok0, e_hi = lim_hi - tok0;  // visible columns
-        const int bad = sc.bad;
-        const bool plain = __all_sync(0xffffffffu, e_lo <= 0 && e_hi >= kPcTok && !bad);
-        // ---- the tile's maxima of x and of x + log2(vs).  Reads of TMEM are slow
-        // while the tensor core works for the other row tile: one wait for all of S.
-        // Its last quarter is read again later, to free registers in between.
-        uint32_t s[4][32];
+        const int bad = sc.bad >> g0;
+        const bool plain = __all_sync(0xffffffffu, e_lo <= 0 && e_hi >= kPcSub && !(bad & 15));
+        // twice in the code, so that the usual subtile has no trace of the masks
+        auto subtile = [&](auto masked) {
+          // ---- the subtile's maxima of x and of x + log2(vs)
+          uint32_t s[2][32];
+          umma::tmem_ld32(t_b, s[0]);
+          umma::tmem_ld32(t_b + 32, s[1]);
+          umma::tmem_wait_ld32(s[0]);
+          umma::tmem_loaded32(s[1]);
+          if constexpr (decltype(masked)::value) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) umma::tmem_ld32(t_s + 32 * c, s[c]);
-        umma::tmem_wait_ld();
-        auto hide = [&](int c) {
-          if (!plain) {
+            for (int e = 0; e < kPcSub; ++e)
+              if (e < e_lo || e >= e_hi || (bad >> (e >> 4) & 1)) s[e >> 5][e & 31] = 0xff800000u;  // -inf
+          }
+          float tm = -INFINITY, tv = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int col = 32 * c + e;
-              if (col < e_lo || col >= e_hi || (bad >> (col >> 4) & 1)) s[c][e] = 0xff800000u;  // -inf
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t* v = s[g >> 1] + 16 * (g & 1);
+            float b0 = __uint_as_float(v[0]), b1 = __uint_as_float(v[1]);
+#pragma unroll
+            for (int e = 2; e < 14; e += 4) {
+              b0 = max3(b0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+              b1 = max3(b1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
             }
+            b0 = max3(b0, __uint_as_float(v[14]), __uint_as_float(v[15]));
+            const float x = fmaxf(b0, b1) * fmaxf(sc.ks[g0 + g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
+            tm = fmaxf(tm, x);
+            tv = fmaxf(tv, x + sc.lv[g0 + g]);
           }
-        };
-        float tm = -INFINITY, tv = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          if (g % 2 == 0) hide(g / 2);
-          const uint32_t* v = s[g >> 1] + 16 * (g & 1);
-          float b0 = __uint_as_float(v[0]), b1 = __uint_as_float(v[1]);
-#pragma unroll
-          for (int e = 2; e < 14; e += 4) {
-            b0 = max3(b0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-            b1 = max3(b1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-          }
-          b0 = max3(b0, __uint_as_float(v[14]), __uint_as_float(v[15]));
-          const float x = fmaxf(b0, b1) * fmaxf(sc.ks[g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
-          tm = fmaxf(tm, x);
-          tv = fmaxf(tv, x + sc.lv[g]);
-        }
-        const bool grew = tm > m + 8.f || tv > mv + 8.f;
-        if (__any_sync(0xffffffffu, grew)) {
-          const float nm = grew ? fmaxf(m, tm) : m, nv = grew ? fmaxf(mv, tv) : mv;
-          if (m != -INFINITY) l *= exp2_fast(m - nm);
-          const float f = mv == -INFINITY ? 1.f : exp2_fast(mv - nv);
-          m = nm;
-          mv = nv;
-          if (i > 0) {
+          const bool grew = tm > m + 8.f || tv > mv + 8.f;
+          if (__any_sync(0xffffffffu, grew)) {
+            const float nm = grew ? fmaxf(m, tm) : m, nv = grew ? fmaxf(mv, tv) : mv;
+            if (m != -INFINITY) l *= exp2_fast(m - nm);
+            const float f = mv == -INFINITY ? 1.f : exp2_fast(mv - nv);
+            m = nm;
+            mv = nv;
+            if (u > 0) {
+              ok = wait(&of[w], (u - 1) & 1);  // the product before may still be under way
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) return;
+              umma::fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D / 8; ++c) {  // few registers: S is held meanwhile
-              uint32_t u[8];
-              umma::tmem_ld8(t_o + 8 * c, u);
-              umma::tmem_wait_ld();
+              for (int c = 0; c < D / 8; ++c) {  // few registers: S is held meanwhile
+                uint32_t u[8];
+                umma::tmem_ld8(t_o + 8 * c, u);
+                umma::tmem_wait_ld8(u);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-              umma::tmem_st8(t_o + 8 * c, u);
+                for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+                umma::tmem_st8(t_o + 8 * c, u);
+              }
+              umma::tmem_wait_st();
             }
-            umma::tmem_wait_st();
           }
-        }
-        // ---- weights: p vs 2^(m - mv) = 2^(x - m + d), d = log2(vs) + m - mv, d >= -100
-        // (a smaller scale's values are nothing beside the row's largest); their sum
-        // over a page's tokens, times 2^-d, goes to l
-        const float base = m == -INFINITY ? 0.f : -m;
-        const float dm = mv == -INFINITY ? 0.f : m - mv;
+          // ---- weights: p vs 2^(m - mv) = 2^(x - m + d), d = log2(vs) + m - mv, d >= -100
+          // (a smaller scale's values are nothing beside the row's largest); their sum
+          // over a page's tokens, times 2^-d, goes to l
+          const float base = m == -INFINITY ? 0.f : -m;
+          const float dm = mv == -INFINITY ? 0.f : m - mv;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c == 1) umma::tmem_ld32(t_s + 96, s[3]);  // P stays below column 64
-          if (c == 3) {
-            umma::tmem_wait_ld();
-            hide(3);
-          }
-          uint32_t p16[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p16[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float cg = fmaxf(sc.ks[2 * c + g] * cq, 0x1p-126f);
-            const float d = fmaxf(sc.lv[2 * c + g] + dm, -100.f), bg = base + d;
-            const uint64_t c2 = pack2(cg, cg), b2 = pack2(bg, bg);
-            uint64_t l2 = pack2(0.f, 0.f);
+            for (int g = 0; g < 2; ++g) {
+              const int gg = g0 + 2 * c + g;
+              const float cg = fmaxf(sc.ks[gg] * cq, 0x1p-126f);
+              const float d = fmaxf(sc.lv[gg] + dm, -100.f), bg = base + d;
+              const uint64_t c2 = pack2(cg, cg), b2 = pack2(bg, bg);
+              uint64_t l2 = pack2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float x0, x1;
-              unpack2(fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, b2), &x0, &x1);
-              x0 = exp2_fast(x0);
-              x1 = exp2_fast(x1);
-              l2 = add2(l2, pack2(x0, x1));
-              p16[8 * g + e / 2] = pack_f16(x0, x1);
+              for (int e = 0; e < 16; e += 2) {
+                float x0, x1;
+                unpack2(fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, b2), &x0, &x1);
+                x0 = exp2_fast(x0);
+                x1 = exp2_fast(x1);
+                l2 = add2(l2, pack2(x0, x1));
+                p16[8 * g + e / 2] = pack_f16(x0, x1);
+              }
+              float l0, l1;
+              unpack2(l2, &l0, &l1);
+              l = fmaf(l0 + l1, exp2_fast(-d), l);
             }
-            float l0, l1;
-            unpack2(l2, &l0, &l1);
-            l = fmaf(l0 + l1, exp2_fast(-d), l);
+            umma::tmem_st16(t_b + 16 * c, p16);
           }
-          umma::tmem_st16(t_s + 16 * c, p16);
-        }
-        umma::tmem_wait_st();
-        umma::fence_before_sync();
-        umma::mbar_arrive(pf + w);
+          umma::tmem_wait_st();
+          umma::fence_before_sync();
+          umma::mbar_arrive(&pf[w][b]);
+        };
+        if (plain) subtile(std::false_type());
+        else subtile(std::true_type());
+        if (!ok) break;
       }
       it += n;
+      tc += n;
       if (!ok) break;
       // ---- the row's result, or this CTA's record of it
-      ok = wait(of + w, uc & 1);
+      // the last two of an even number of products (a phase is told from the one
+      // before it only, and the last but one may still be under way)
+      ok = wait(&of[w], 0) && wait(&of[w], 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      ++uc;
       umma::fence_after_sync();
       const int R = pc.row0 + 128 * w + r, tok_q = R / rq.G, head = pc.h * rq.G + R % rq.G;
       const bool whole = pc.whole, live = R < pc.rows;
@@ -587,7 +601,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         umma::tmem_ld32(t_o + 32 * c, o);
-        umma::tmem_wait_ld();
+        umma::tmem_wait_ld32(o);
         if (live) {
           if (whole) {
 #pragma unroll
