@@ -20,7 +20,7 @@
 // Two references per row, in base 2: m for the sum l of the weights, and mv
 // for O, whose weights carry the page's value scale: p vs = 2^(x - m) (vs 2^(m -
 // mv)), so the f16 rounding of P is relative to the largest p vs.  They follow
-// the running maxima only when these pass them by 8 (P <= 2^8): rescaling O,
+// the running maxima only when these pass them by 14 (P <= 2^14): rescaling O,
 // which lies in TMEM, is rare after the first tiles.
 //
 // Q is scaled per row by a power of two and rounded to f16 (exact but for
@@ -48,6 +48,7 @@ constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
 constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
+constexpr float kPcSlack = 14.f;           // log2 of the largest P: below f16's 2^16
 constexpr long kPcPolls = 1L << 20;
 
 struct ChunkArgs {
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   __shared__ ChunkScales scales[L::ring];
   __shared__ uint64_t kf[NS], ke[NS], vf[NS], ve[NS];  // a stage of keys, of values: full, empty
   __shared__ uint64_t sf[2][2], pf[2][2];              // scores, weights of (row tile, S buffer)
-  __shared__ uint64_t of[2], qf, drain;                // a subtile's product into O of a row tile; queries
+  __shared__ uint64_t of[2], od[2], qf, drain;         // a subtile's product into O, a unit's last one; queries
   __shared__ uint64_t nf[kPcPieces], ne[kPcPieces];    // pieces
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
@@ -148,6 +149,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         umma::mbar_init(&pf[w][b], 128);
       }
       umma::mbar_init(of + w, 1);
+      umma::mbar_init(od + w, 1);
     }
     for (int i = 0; i < kPcPieces; ++i) {
       umma::mbar_init(nf + i, 1);
@@ -279,6 +281,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           if (more) commit(ke + nx);
         }
         if (!ok) break;
+        commit(od);
+        if (two) commit(od + 1);
         it += n;
       }
       if (!ok) {  // nothing may be in flight when TMEM is freed
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     const int w = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t t_s = tmem + 128 * w + lanes, t_o = tmem + 256 + D * w + lanes;
-    int it = 0, tc = 0;
+    int it = 0, tc = 0, uc = 0;  // tiles of all units and of this row tile, units of it
     bool ok = true;
     for (int un = 0;; ++un) {
       const int sl = un % kPcPieces;
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             tm = fmaxf(tm, x);
             tv = fmaxf(tv, x + sc.lv[g0 + g]);
           }
-          const bool grew = tm > m + 8.f || tv > mv + 8.f;
+          const bool grew = tm > m + kPcSlack || tv > mv + kPcSlack;
           if (__any_sync(0xffffffffu, grew)) {
             const float nm = grew ? fmaxf(m, tm) : m, nv = grew ? fmaxf(mv, tv) : mv;
             if (m != -INFINITY) l *= exp2_fast(m - nm);
@@ -525,18 +529,21 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             m = nm;
             mv = nv;
             if (u > 0) {
-              ok = wait(&of[w], (u - 1) & 1);  // the product before may still be under way
+              // The product before may still be under way.  The one before that is done
+            // (S of this subtile came after it) and the next waits for this thread, so
+            // the phase's parity says which it is.
+            ok = wait(&of[w], (u - 1) & 1);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) return;
               umma::fence_after_sync();
 #pragma unroll 1
-              for (int c = 0; c < D / 8; ++c) {  // few registers: S is held meanwhile
-                uint32_t u[8];
-                umma::tmem_ld8(t_o + 8 * c, u);
-                umma::tmem_wait_ld8(u);
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                umma::tmem_ld32(t_o + 32 * c, o);
+                umma::tmem_wait_ld32(o);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-                umma::tmem_st8(t_o + 8 * c, u);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                umma::tmem_st32(t_o + 32 * c, o);
               }
               umma::tmem_wait_st();
             }
@@ -583,11 +590,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       tc += n;
       if (!ok) break;
       // ---- the row's result, or this CTA's record of it
-      // the last two of an even number of products (a phase is told from the one
-      // before it only, and the last but one may still be under way)
-      ok = wait(&of[w], 0) && wait(&of[w], 1);
+      ok = wait(&od[w], uc & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      ++uc;
       umma::fence_after_sync();
       const int R = pc.row0 + 128 * w + r, tok_q = R / rq.G, head = pc.h * rq.G + R % rq.G;
       const bool whole = pc.whole, live = R < pc.rows;
