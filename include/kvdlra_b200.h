@@ -309,7 +309,8 @@ int kvd_page_tables(int32_t batch, int32_t max_pages, int32_t page_size, const i
                     const int32_t* new_lens, int32_t* table, int64_t table_stride,
                     const int32_t* free_pages, int32_t num_free, const int32_t* free_count, int32_t capacity,
                     int32_t* lens, int32_t* free_left, int32_t* cu_new, int32_t* slots, int32_t* positions,
-                    int32_t* status, kvd_stream_t stream);
+                    int32_t* status, void* workspace, size_t ws_bytes, kvd_stream_t stream);
+size_t kvd_page_tables_workspace_bytes(int32_t batch, int32_t capacity); /* 0: none is needed */
 /* Requests with done[b] != 0 give their pages back on top of the free stack,
  * in request order, and have lens[b] = 0 afterwards. */
 int kvd_page_release(int32_t batch, int32_t max_pages, int32_t page_size, const uint8_t* done, int32_t* lens,

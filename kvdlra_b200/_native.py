@@ -157,7 +157,9 @@ def lib() -> C.CDLL:
     L.kvd_blocked_project.argtypes = [i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, sz, vp]
     L.kvd_blocked_project_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.kvd_blocked_project_workspace_bytes.restype = sz
-    L.kvd_page_tables.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+    L.kvd_page_tables.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.kvd_page_tables_workspace_bytes.argtypes = [i32, i32]
+    L.kvd_page_tables_workspace_bytes.restype = sz
     L.kvd_page_release.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, vp, vp]
     L.kvd_paged_append.argtypes = [P(PagedPool), vp, i32, i32, HFView, HFView, vp]
     L.kvd_paged_peek.argtypes = [P(PagedPool), i32, vp, i64, i32, vp, i32, HFView, HFView, vp]

@@ -272,6 +272,13 @@ struct PagedPart {
   int4* head;          // [ctas]: request, KV head, row tile, pieces (0: none)
 };
 
+// A row's weights before their rounding to f16: P = p vs / 2^mv.  The reference
+// mv is kPBias under the largest p vs when it is set and moves when P would pass
+// 2^kPTop: P's subnormals, spaced 2^-24, are 2^-30 of the row's largest weight or
+// less, and the move, which rescales O, is rare after the first tiles.
+constexpr float kPBias = 6.f, kPTop = 15.f;
+constexpr float kLTop = 14.f;  // log2 of the largest weight in l, over its own reference m
+
 KVD_DEVICE float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -290,10 +297,18 @@ struct PagedOut {
 };
 
 // Joins a split unit's records: M = max m_i, out = sum 2^(m_i - M) O_i / sum
-// 2^(m_i - M) l_i.  One CTA per (CTA of the kernel above, slice of the rows);
-// most have nothing to do.  Bound by the latency of reading the records.
+// 2^(m_i - M) l_i.  blockIdx.x is the CTA of the kernel before that began the
+// unit (most began none that others finish); the rows go over blockIdx.y and the
+// warps.  A row is a warp's, or the four warps' where there are many records (a
+// long context split over the SMs): the lanes find the records' factors, one
+// each, then every lane sums its columns over them.  Bound by the latency of a
+// few dependent reads: 4 us for 64 records, where one pass for the maximum and one
+// for the sums, a thread per column, took 41.
 template <int D, int RT, typename T>
 __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPart part, PagedOut out, int fill_tail) {
+  constexpr int V = D < 128 ? D / 32 : 4;      // columns per lane and step
+  constexpr int C = D / (32 * V);              // steps
+  __shared__ float sums[4][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (fill_tail && rq.cu_q) {  // rows behind the last request: zeros
     const long from = (long)max(0, min(rq.cu_q[rq.batch], rq.q_tokens)) * out.Hq, to = (long)rq.q_tokens * out.Hq;
@@ -305,30 +320,81 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPar
   }
   const int4 u = part.head[blockIdx.x];
   if (u.w == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = u.x, h = u.y, rt = u.z, n = u.w;
   const int rows = min(RT, rq.q_len(b) * rq.G - rt * RT);
   const long step = 2L * RT * (D + 2);
-  const float* r0 = part.rec + (long)blockIdx.x * step + (long)RT * (D + 2);  // record 1 of the first CTA
-  const float* r1 = part.rec + (long)(blockIdx.x + 1) * step;                 // record 0 of those after it
-  for (int e = blockIdx.y * 128 + threadIdx.x; e < rows * D; e += gridDim.y * 128) {
-    const int r = e / D, d = e % D;
-    float M = r0[RT * D + r];
-#pragma unroll 8
-    for (int i = 0; i < n - 1; ++i) M = fmaxf(M, r1[i * step + RT * D + r]);
-    const float f = M == -INFINITY ? 1.f : exp2_fast(r0[RT * D + r] - M);
-    float L = f * r0[RT * D + RT + r], o = f * r0[r * D + d];
-#pragma unroll 8
-    for (int i = 0; i < n - 1; ++i) {
-      const float* p = r1 + i * step;
-      const float w = M == -INFINITY ? 1.f : exp2_fast(p[RT * D + r] - M);
-      L = fmaf(w, p[RT * D + RT + r], L);
-      o = fmaf(w, p[r * D + d], o);
+  // record 1 of the CTA that began the unit, then record 0 of those after it
+  const float* first = part.rec + (long)blockIdx.x * step + (long)RT * (D + 2);
+  const float* rest = part.rec + (long)blockIdx.x * step;
+  auto record = [&](int i) { return i == 0 ? first : rest + i * step; };
+  const bool many = n >= 12;
+  const int per = many ? 1 : 4, stride = many ? 4 : 1, part0 = many ? warp : 0;
+  for (int r = blockIdx.y * per + (many ? 0 : warp); r < rows; r += gridDim.y * per) {
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, record(i)[RT * D + r]);
+    M = warp_max(M);
+    float L = 0.f, o[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[c][k] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float f = 0.f;
+      if (i0 + lane < n) {
+        const float* p = record(i0 + lane);
+        f = M == -INFINITY ? 1.f : exp2_fast(p[RT * D + r] - M);
+        L = fmaf(f, p[RT * D + RT + r], L);
+      }
+      const int m = min(32, n - i0);
+#pragma unroll 4
+      for (int i = part0; i < m; i += stride) {
+        const float w = __shfl_sync(0xffffffffu, f, i);
+        const float* p = record(i0 + i) + r * D + V * lane;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float x[V];
+          if constexpr (V == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(p + 128 * c);
+            x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+          } else if constexpr (V == 2) {
+            const float2 y = *reinterpret_cast<const float2*>(p);
+            x[0] = y.x; x[1] = y.y;
+          } else {
+            x[0] = *p;
+          }
+#pragma unroll
+          for (int k = 0; k < V; ++k) o[c][k] = fmaf(w, x[k], o[c][k]);
+        }
+      }
+    }
+    L = warp_sum(L);
+    if (many) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sums[warp][32 * V * c + V * lane + k] = o[c][k];
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const int d = 32 * V * c + V * lane + k;
+          o[c][k] = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+        }
+      __syncthreads();
+      if (warp != 0) continue;
     }
     const int R = rt * RT + r;
     const long row = (rq.cu_q ? rq.q0(b) : (long)b * rq.q_tokens) + R / rq.G;
     const int hq = h * rq.G + R % rq.G;
-    store_f(reinterpret_cast<T*>(out.out) + (row * out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
-    if (d == 0 && out.lse) out.lse[row * out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    T* dst = reinterpret_cast<T*>(out.out) + (row * out.Hq + hq) * D + V * lane;
+    const float f = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int k = 0; k < V; ++k) store_f(dst + 32 * V * c + k, o[c][k] * f);
+    if (lane == 0 && out.lse) out.lse[row * out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
   }
 }
 
@@ -362,7 +428,7 @@ int launch_merge(const PagedReqs& rq, const PagedPart& part, const PagedOut& out
                         cudaStream_t s) {
   // starts while the kernel before it drains, and waits for it in the kernel
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, (RT * D + 511) / 512);
+  cfg.gridDim = dim3(ctas, RT < 32 ? RT : 32);
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at[1];

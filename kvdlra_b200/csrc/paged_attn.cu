@@ -28,7 +28,7 @@
 // Two references per row, in base 2: m for the sum l of the weights, and mv
 // for O, whose weights carry the page's value scale: p vs = 2^(x - m) (vs
 // 2^(m - mv)), so P's rounding is relative to the largest p vs.  They follow
-// the running maxima only when these pass them by 8 (P <= 2^8): a tile costs
+// the running maxima only when these pass them by kLTop and kPTop: a tile costs
 // one vote instead of reductions over the lanes.
 //
 // Work: (request, KV head, row tile, 128-token tile) is one list, every CTA
@@ -327,14 +327,14 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) grew |= mt[nt][c] > m[nt][c] + 8.f || vt[nt][c] > mv[nt][c] + 8.f;
+          for (int c = 0; c < 2; ++c) grew |= mt[nt][c] > m[nt][c] + kLTop || vt[nt][c] > mv[nt][c] + kPTop;
         if (__any_sync(0xffffffffu, grew)) {  // rare after the first tiles
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float al[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float x = fmaxf(m[nt][c], mt[nt][c]), y = fmaxf(mv[nt][c], vt[nt][c]);
+              float x = fmaxf(m[nt][c], mt[nt][c]), y = fmaxf(mv[nt][c], vt[nt][c] - kPBias);
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) {
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -524,7 +524,7 @@ int paged_pool_view(const kvd_paged_pool* p, PagedPool* out) {
 
 // A request of at most this many rows goes to the few-row kernel: its codes are
 // read once per 8 or 16 rows, the tensor-memory kernel's once per 256.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 16;
 
 // rows per unit of the few-row kernel: eight, or sixteen for longer groups
 // (head_dim 256: sixteen rows' accumulators would not fit the registers)

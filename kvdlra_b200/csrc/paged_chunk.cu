@@ -20,7 +20,7 @@
 // Two references per row, in base 2: m for the sum l of the weights, and mv
 // for O, whose weights carry the page's value scale: p vs = 2^(x - m) (vs 2^(m -
 // mv)), so the f16 rounding of P is relative to the largest p vs.  They follow
-// the running maxima only when these pass them by 14 (P <= 2^14): rescaling O,
+// the running maxima only when these pass them by kLTop and kPTop: rescaling O,
 // which lies in TMEM, is rare after the first tiles.
 //
 // Q is scaled per row by a power of two and rounded to f16 (exact but for
@@ -48,7 +48,6 @@ constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
 constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
-constexpr float kPcSlack = 14.f;           // log2 of the largest P: below f16's 2^16
 constexpr long kPcPolls = 1L << 20;
 
 struct ChunkArgs {
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   __shared__ ChunkScales scales[L::ring];
   __shared__ uint64_t kf[NS], ke[NS], vf[NS], ve[NS];  // a stage of keys, of values: full, empty
   __shared__ uint64_t sf[2][2], pf[2][2];              // scores, weights of (row tile, S buffer)
-  __shared__ uint64_t of[2], od[2], qf, drain;         // a subtile's product into O, a unit's last one; queries
+  __shared__ uint64_t of[2], od[2], qf[2], drain;      // a subtile's product into O, a unit's last one; queries
   __shared__ uint64_t nf[kPcPieces], ne[kPcPieces];    // pieces
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
@@ -150,12 +149,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       }
       umma::mbar_init(of + w, 1);
       umma::mbar_init(od + w, 1);
+      umma::mbar_init(qf + w, 128);
     }
     for (int i = 0; i < kPcPieces; ++i) {
       umma::mbar_init(nf + i, 1);
       umma::mbar_init(ne + i, 256 + 256 + 1);
     }
-    umma::mbar_init(&qf, 256);
     umma::mbar_init(&drain, 1);
     umma::mbar_fence_init();
   }
@@ -231,7 +230,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         __syncwarp();
       };
       auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-      int it = 0, t0 = 0, t1 = 0;  // tiles so far, of all units and by row tile
+      int it = 0, t0 = 0, t1 = 0, un1 = 0;  // tiles so far, of all units and by row tile; units of the second
       bool ok = true;
       for (int un = 0;; ++un) {
         const int sl = un % kPcPieces;
@@ -241,7 +240,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         const bool two = __shfl_sync(0xffffffffu, pieces[sl].rows - pieces[sl].row0 > 128, 0);
         if (lane == 0) umma::mbar_arrive(ne + sl);
         if (n == 0) break;
-        ok = wait_all(&qf, un & 1) && wait_all(kf + it % NS, (it / NS) & 1);
+        // a row tile that has no rows takes no part: its threads may be units ahead
+        ok = wait_all(qf, un & 1) && (!two || wait_all(qf + 1, un1++ & 1)) && wait_all(kf + it % NS, (it / NS) & 1);
         if (!ok) break;
         umma::fence_after_sync();
         for (int b = 0; b < 2; ++b) {
@@ -473,9 +473,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           *reinterpret_cast<uint4*>(dst + (c >> 3) * kPcBlock + 16 * ((c & 7) ^ (r & 7))) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         umma::fence_proxy_async_smem();
-      }
-      umma::mbar_arrive(&qf);
-      if (!active) {
+        umma::mbar_arrive(qf + w);
+      } else {
         umma::mbar_arrive(ne + sl);
         it += n;
         continue;
@@ -521,9 +520,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
             tm = fmaxf(tm, x);
             tv = fmaxf(tv, x + sc.lv[g0 + g]);
           }
-          const bool grew = tm > m + kPcSlack || tv > mv + kPcSlack;
+          const bool grew = tm > m + kLTop || tv > mv + kPTop;
           if (__any_sync(0xffffffffu, grew)) {
-            const float nm = grew ? fmaxf(m, tm) : m, nv = grew ? fmaxf(mv, tv) : mv;
+            const float nm = grew ? fmaxf(m, tm) : m, nv = grew ? fmaxf(mv, tv - kPBias) : mv;
             if (m != -INFINITY) l *= exp2_fast(m - nm);
             const float f = mv == -INFINITY ? 1.f : exp2_fast(mv - nv);
             m = nm;

@@ -35,7 +35,8 @@ struct AppendArgs {
 constexpr int kMaxPage = 128;
 
 template <int D, int W, int STORE, typename T>
-__global__ void __launch_bounds__(W < 4 ? 128 : 32 * W) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 : 512) / (W < 4 ? 128 : 32 * W))
+    paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int NTHR = W < 4 ? 128 : 32 * W;      // threads of the CTA
   constexpr int GT = 32 * W, GROUPS = NTHR / GT;  // threads of a group, groups (heads) of the CTA
   constexpr int VE = 16 / (int)sizeof(T);         // elements per load

@@ -8,12 +8,13 @@
 // exclusive prefix sum of t, at position p = c_b + i - cu_b and slot
 // table[b][p / S] * S + p % S.  Rows behind the last request get slot -1.
 //
-// A few integers per request and row: latency bounds it.  One launch: a
-// cluster of one or eight CTAs, each of which scans all requests for itself
-// (a few reads per thread) and then takes its share of the new pages and of
-// the rows; cluster barriers stand between the reads of the lengths, the
-// table's new entries, the rows that use them, and the writes of what may
-// alias the inputs.
+// A few integers per request and row: latency bounds it, the writes of slots and
+// positions where there are a million rows.  A small step is one launch of one
+// CTA.  A larger one is two: one CTA scans the requests, then a grid takes the
+// rows and the table's new entries; a row's page is looked up in the table or on
+// the stack, whichever holds it, so the grid's CTAs need nothing of one another.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace kvd {
@@ -36,11 +37,8 @@ struct TableArgs {
   int* slots;
   int* positions;
   int* status;
+  int* pages_before;  // [batch + 1], two launches
 };
-
-KVD_DEVICE void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // largest b with pre[b] <= x (pre ascending, pre[0] = 0, x < pre[n])
 KVD_DEVICE int find_owner(const int* pre, int n, int x) {
@@ -52,20 +50,66 @@ KVD_DEVICE int find_owner(const int* pre, int n, int x) {
   return lo;
 }
 
+// The table's new entries and the rows, by `threads` threads, `me` one of them.
+// cu and pp (new pages of the requests before) in any memory, cached(b) the tokens
+// held, top the free count before the step.
+template <typename F>
+KVD_DEVICE void table_rows(const TableArgs& a, const int* cu, const int* pp, F cached, int top, int rows, int pages, long me, long threads) {
+  const int mask = (1 << a.lg_page) - 1;
+  for (long e = me; e < pages; e += threads) {
+    const int b = find_owner(pp, a.batch, (int)e);
+    const int have = (cached(b) + mask) >> a.lg_page;
+    a.table[(long)b * a.table_stride + have + (e - pp[b])] = a.free_pages[top - 1 - e];
+  }
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
+  for (long r0 = 4 * me; r0 < a.capacity; r0 += 4 * threads) {  // four neighbours a thread
+    int s[4], q[4];
+    int b = r0 < rows ? find_owner(cu, a.batch, (int)r0) : 0;
+    int next = r0 < rows ? cu[b + 1] : 0, c_of = -1, c = 0, begin = 0, page_no = -1, id = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (int)r0 + i;
+      s[i] = -1;
+      q[i] = 0;
+      if (r < rows) {
+        while (next <= r) next = cu[++b + 1];
+        if (b != c_of) { c_of = b; c = cached(b); begin = cu[b]; page_no = -1; }
+        q[i] = c + r - begin;
+        const int pn = q[i] >> a.lg_page;
+        if (pn != page_no) {
+          page_no = pn;
+          const int have = (c + mask) >> a.lg_page;
+          id = pn < have ? a.table[(long)b * a.table_stride + pn] : a.free_pages[top - 1 - (pp[b] + pn - have)];
+        }
+        s[i] = (id << a.lg_page) + (q[i] & mask);
+      }
+    }
+    if (wide && r0 + 4 <= a.capacity) {
+      *reinterpret_cast<int4*>(a.slots + r0) = make_int4(s[0], s[1], s[2], s[3]);
+      *reinterpret_cast<int4*>(a.positions + r0) = make_int4(q[0], q[1], q[2], q[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + i < a.capacity) { a.slots[r0 + i] = s[i]; a.positions[r0 + i] = q[i]; }
+    }
+  }
+}
+
+// The scan, by one CTA; with ALL the rest of the step too.
+template <bool ALL>
 __global__ void __launch_bounds__(kTabThreads) paged_tables_kernel(const __grid_constant__ TableArgs a) {
   extern __shared__ int tsm[];
   int* cu = tsm;                    // [batch + 1]
   int* pp = tsm + a.batch + 1;      // [batch + 1] new pages of the requests before
   __shared__ long wsum[2][32];
   __shared__ int bad_sm;
+  if constexpr (!ALL) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t rank, ctas;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
   if (tid == 0) bad_sm = 0;
   const int mask = (1 << a.lg_page) - 1;
   const int per = (a.batch + kTabThreads - 1) / kTabThreads;
   const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+  const int free_count = *a.free_count;
   long st = 0, sp = 0;
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
@@ -82,7 +126,6 @@ __global__ void __launch_bounds__(kTabThreads) paged_tables_kernel(const __grid_
     if (lane >= o) { it += yt; ip += yp; }
   }
   if (lane == 31) { wsum[0][warp] = it; wsum[1][warp] = ip; }
-  const int free_count = *a.free_count;
   __syncthreads();
   long bt = 0, bp = 0, rows = 0, pages = 0;
 #pragma unroll 8
@@ -94,67 +137,44 @@ __global__ void __launch_bounds__(kTabThreads) paged_tables_kernel(const __grid_
   if (bad || rows > a.capacity || pages > free_count || free_count > a.num_free) bad_sm = 1;
   __syncthreads();
   const bool ok = bad_sm == 0;
-  if (ok) {
+  if (!ok) rows = pages = 0;
+  {
     int t = (int)(bt + it - st), p = (int)(bp + ip - sp);
     for (int b = b0; b < b1; ++b) {
-      cu[b] = t;
-      pp[b] = p;
       const int c = a.cached[b], n = a.added[b];
-      t += n;
-      p += ((c + n + mask) >> a.lg_page) - ((c + mask) >> a.lg_page);
-    }
-    if (tid == 0) { cu[a.batch] = (int)rows; pp[a.batch] = (int)pages; }
-    __syncthreads();
-    // ---- new table entries
-    for (int e = rank * kTabThreads + tid; e < (int)pages; e += ctas * kTabThreads) {
-      const int b = find_owner(pp, a.batch, e);
-      const int have = (a.cached[b] + mask) >> a.lg_page;
-      a.table[(long)b * a.table_stride + have + (e - pp[b])] = a.free_pages[free_count - 1 - e];
-    }
-  }
-  cluster_barrier();  // the entries are there for every CTA
-  // ---- the step's rows, four neighbours a thread
-  for (long r0 = 4L * (rank * kTabThreads + tid); r0 < a.capacity; r0 += 4L * ctas * kTabThreads) {
-    int s[4], q[4];
-    int b = ok && r0 < rows ? find_owner(cu, a.batch, (int)r0) : 0;
-    int page_no = -1, page_b = -1, id = 0, c = 0, c_of = -1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (int)r0 + i;
-      s[i] = -1;
-      q[i] = 0;
-      if (ok && r < rows) {
-        while (cu[b + 1] <= r) ++b;
-        if (b != c_of) { c = a.cached[b]; c_of = b; }
-        q[i] = c + r - cu[b];
-        if (page_b != b || page_no != (q[i] >> a.lg_page)) {
-          page_b = b;
-          page_no = q[i] >> a.lg_page;
-          id = a.table[(long)b * a.table_stride + page_no];
-        }
-        s[i] = (id << a.lg_page) + (q[i] & mask);
+      cu[b] = ok ? t : 0;
+      pp[b] = ok ? p : 0;
+      if (ok) {
+        t += n;
+        p += ((c + n + mask) >> a.lg_page) - ((c + mask) >> a.lg_page);
       }
     }
-    if (r0 + 4 <= a.capacity && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
-      *reinterpret_cast<int4*>(a.slots + r0) = make_int4(s[0], s[1], s[2], s[3]);
-      *reinterpret_cast<int4*>(a.positions + r0) = make_int4(q[0], q[1], q[2], q[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r0 + i < a.capacity) { a.slots[r0 + i] = s[i]; a.positions[r0 + i] = q[i]; }
-    }
+    if (tid == 0) { cu[a.batch] = (int)rows; pp[a.batch] = (int)pages; }
   }
-  cluster_barrier();  // nobody reads the lengths or the count any more
-  for (int b = rank * kTabThreads + tid; b < a.batch; b += ctas * kTabThreads) {
-    const int c = a.cached[b], n = ok ? a.added[b] : 0;
-    a.cu[b] = ok ? cu[b] : 0;
-    a.lens[b] = c + n;
+  __syncthreads();
+  if constexpr (ALL) {
+    table_rows(a, cu, pp, [&](int b) { return a.cached[b]; }, free_count, (int)rows, (int)pages, tid, kTabThreads);
+    __syncthreads();  // nobody reads the lengths any more
   }
-  if (rank == 0 && tid == 0) {
-    a.cu[a.batch] = ok ? (int)rows : 0;
-    *a.free_left = ok ? free_count - (int)pages : free_count;
+  for (int b = tid; b <= a.batch; b += kTabThreads) {
+    a.cu[b] = cu[b];
+    if constexpr (!ALL) a.pages_before[b] = pp[b];
+    if (b < a.batch) a.lens[b] = a.cached[b] + (ok ? a.added[b] : 0);
+  }
+  if (tid == 0) {
+    *a.free_left = free_count - (int)pages;
     if (!ok && a.status) atomicOr(a.status + kStatusBounds, kPagedNoRoom);
   }
+}
+
+// The rest of a large step, after the scan.  What the scan read may be
+// overwritten by now: the lengths and the count before the step are those after
+// it less what the step added.
+__global__ void __launch_bounds__(256) paged_rows_map_kernel(const __grid_constant__ TableArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int rows = a.cu[a.batch], pages = a.pages_before[a.batch];
+  table_rows(a, a.cu, a.pages_before, [&](int b) { return a.lens[b] - a.added[b]; }, *a.free_left + pages, rows, pages,
+             (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256);
 }
 
 // Requests b with done[b] give their ceil(len / S) pages back, in request
@@ -239,11 +259,15 @@ static int table_checks(const char* what, int batch, int max_pages, int64_t stri
 
 using namespace kvd_host;
 
+extern "C" size_t kvd_page_tables_workspace_bytes(int32_t batch, int32_t capacity) {
+  return (long)capacity + batch <= 8192 || batch < 0 ? 0 : (size_t)(batch + 1) * sizeof(int);
+}
+
 extern "C" int kvd_page_tables(int32_t batch, int32_t max_pages, int32_t page_size, const int32_t* cached_lens,
                                const int32_t* new_lens, int32_t* table, int64_t table_stride,
                                const int32_t* free_pages, int32_t num_free, const int32_t* free_count, int32_t capacity,
                                int32_t* lens, int32_t* free_left, int32_t* cu_new, int32_t* slots, int32_t* positions,
-                               int32_t* status, kvd_stream_t stream) try {
+                               int32_t* status, void* workspace, size_t ws_bytes, kvd_stream_t stream) try {
   if (int rc = table_checks("page tables", batch, max_pages, table_stride, page_size, num_free)) return rc;
   if (capacity < 0 || capacity > INT32_MAX - 8192 * 4) { set_error("page tables: capacity %d", capacity); return KVD_ERR_ARG; }
   if (!cached_lens || !new_lens || !table || (!free_pages && num_free) || !free_count || !lens || !free_left || !cu_new ||
@@ -252,25 +276,41 @@ extern "C" int kvd_page_tables(int32_t batch, int32_t max_pages, int32_t page_si
     return KVD_ERR_ARG;
   }
   kvd::TableArgs a{batch, max_pages, lg_of(page_size), num_free, capacity, cached_lens, new_lens, table, (long)table_stride,
-                   free_pages, free_count, lens, free_left, cu_new, slots, positions, status};
+                   free_pages, free_count, lens, free_left, cu_new, slots, positions, status, (int*)workspace};
   const size_t smem = 2 * (size_t)(batch + 1) * sizeof(int);
-  if (int rc = ensure_smem((const void*)kvd::paged_tables_kernel, smem, "paged_tables_kernel")) return rc;
-  // one CTA finishes a few thousand rows sooner than a cluster's barriers cost
-  const int ctas = (long)capacity + batch <= 8192 ? 1 : 8;
+  const cudaStream_t s = (cudaStream_t)stream;
+  // One CTA takes about 4 us for each 4096 rows; from twice that on a second
+  // launch, which spreads them over the SMs, costs less.
+  const bool one = (long)capacity + batch <= 8192;
+  const void* scan = one ? (const void*)kvd::paged_tables_kernel<true> : (const void*)kvd::paged_tables_kernel<false>;
+  if (smem > 48 * 1024)
+    if (int rc = ensure_smem(scan, smem, "paged_tables_kernel")) return rc;
+  if (one) {
+    KTimerScope kts_("paged_tables_kernel", s);
+    kvd::paged_tables_kernel<true><<<1, kvd::kTabThreads, smem, s>>>(a);
+    return check_launch("paged_tables_kernel");
+  }
+  if (!workspace || ws_bytes < kvd_page_tables_workspace_bytes(batch, capacity)) {
+    set_error("page tables: workspace of %zu bytes is needed", kvd_page_tables_workspace_bytes(batch, capacity));
+    return KVD_ERR_WORKSPACE;
+  }
+  {
+    KTimerScope kts_("paged_tables_kernel", s);
+    kvd::paged_tables_kernel<false><<<1, kvd::kTabThreads, smem, s>>>(a);
+  }
+  if (int rc = check_launch("paged_tables_kernel")) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kvd::kTabThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)stream;
+  cfg.gridDim = dim3((unsigned)std::max(1L, std::min(4L * paged_sm_count(), ((long)capacity + 1023) / 1024)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ctas;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  KTimerScope kts_("paged_tables_kernel", (cudaStream_t)stream);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kvd::paged_tables_kernel, a);
-  if (e != cudaSuccess) { set_error("paged_tables_kernel: %s", cudaGetErrorString(e)); return KVD_ERR_CUDA; }
+  KTimerScope kts_("paged_rows_map_kernel", s);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kvd::paged_rows_map_kernel, a);
+  if (e != cudaSuccess) { set_error("paged_rows_map_kernel: %s", cudaGetErrorString(e)); return KVD_ERR_CUDA; }
   return KVD_OK;
 } catch (...) {
   set_error("page tables: host error");

@@ -215,15 +215,19 @@ def build_page_tables(cached_lens: Tensor, new_lens: Tensor, table: Tensor, free
     _cuda(device)
     # one allocation: slots and positions first, both on 16-byte borders
     cap = (capacity + 3) & ~3
-    buf = torch.empty(2 * cap + 2 * batch + 2, dtype=torch.int32, device=device)
+    lib = N.lib()
+    ws = lib.kvd_page_tables_workspace_bytes(batch, capacity)
+    n = 2 * cap + 2 * batch + 2
+    buf = torch.empty(n + ws // 4, dtype=torch.int32, device=device)
     slots, positions = buf[:capacity], buf[cap : cap + capacity]
     cu = buf[2 * cap : 2 * cap + batch + 1]
     lens = cached_lens if in_place else buf[2 * cap + batch + 1 : 2 * cap + 2 * batch + 1]
-    left = free_count if in_place else buf[2 * cap + 2 * batch + 1 :]
-    _call(device, N.lib().kvd_page_tables, "kvd_page_tables", batch, table.shape[1], page_size, cached_lens.data_ptr(),
+    left = free_count if in_place else buf[n - 1 : n]
+    _call(device, lib.kvd_page_tables, "kvd_page_tables", batch, table.shape[1], page_size, cached_lens.data_ptr(),
           new_lens.data_ptr(), table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.shape[0],
           free_count.data_ptr(), capacity, lens.data_ptr(), left.data_ptr(), cu.data_ptr(), slots.data_ptr(),
-          positions.data_ptr(), None if status is None else status.data_ptr(), _stream(device.index))
+          positions.data_ptr(), None if status is None else status.data_ptr(), buf.data_ptr() + 4 * n if ws else None, ws,
+          _stream(device.index))
     return PagePlan(lens, cu, slots, positions, left)
 
 

@@ -86,14 +86,16 @@ def dense(codes, scales, table, n):
     return out
 
 
-def attention(q, k, v, scaling, window=0, start=0):
-    """q (n, Hq, D), k and v (H, len, D), all float64.  Returns out (n, Hq, D),
-    lse (n, Hq), and what the error bounds are made of: weight (n, Hq, D) = sum
-    w |v|, and size (n, Hq) = the largest scaling * sum |q_d k_d| a row sees."""
+def attention(q, k, v, scaling, window=0, start=0, vs=None):
+    """q (n, Hq, D), k and v (H, len, D), all float64, vs (H, len) the values'
+    scale of each token.  Returns out (n, Hq, D), lse (n, Hq), and what the error
+    bounds are made of: weight (n, Hq, D) = sum w |v|, size (n, Hq) = the largest
+    scaling * sum |q_d k_d| a row sees, flush (n, Hq, D) = max(w vs) sum |v| / vs
+    (0 without vs)."""
     n, hq, dim = q.shape
     heads, length = k.shape[:2]
     out, lse = np.zeros(q.shape), np.full((n, hq), -np.inf)
-    weight, size = np.zeros(q.shape), np.zeros((n, hq))
+    weight, size, flush = np.zeros(q.shape), np.zeros((n, hq)), np.zeros(q.shape)
     for i in range(n):
         hi = min(length, length - n + i + 1)
         lo = max(start, hi - window) if window else start
@@ -109,24 +111,26 @@ def attention(q, k, v, scaling, window=0, start=0):
             out[i, h] = w @ v[g, lo:hi]
             weight[i, h] = w @ np.abs(v[g, lo:hi])
             size[i, h] = (np.abs(k[g, lo:hi]) @ np.abs(q[i, h])).max() * abs(scaling)
-    return out, lse, weight, size
+            if vs is not None:
+                s = vs[g, lo:hi]
+                flush[i, h] = (w * s).max() * (np.abs(v[g, lo:hi]) / s[:, None]).sum(0)
+    return out, lse, weight, size, flush
 
 
-def bounds(ref, lse, weight, size, dim, length, dtype):
+def bounds(ref, lse, weight, size, flush, dim, length, dtype):
     """How far (out, lse) may be off, elementwise.
 
     Scores: products are exact in fp32 and summed there, dim terms, each sum off
     by at most 2^-23 of the running magnitude; q's split or rounding and the
     scales' products add 2^-22.  A weight is off by that times size, by 2^-21
     from the exponential, and by 2^-11 (16-bit types: one rounding to f16) or
-    2^-21 (fp32: two f16 parts); sums over the tokens add length 2^-23.  Weights
-    under 2^-14 of the largest keep an absolute 2^-25 of it, which the sum over
-    the tokens bounds by length 2^-25 of sum w |v|.  The result's own rounding
-    is half a step."""
+    2^-21 (fp32: two f16 parts); sums over the tokens add length 2^-23.  What is
+    rounded to f16 is w vs; under 2^-14 of its largest value f16 is spaced 2^-24 of
+    that, an absolute error of 2^-25 max(w vs) in w vs, so of 2^-25 flush in the
+    sum over w vs (v / vs).  The result's own rounding is half a step."""
     score = ((dim + 8) * 2.0**-23 + 2.0**-21) * size
     rel = score + 2.0**-21 + length * 2.0**-22 + (2.0**-21 if dtype == torch.float32 else 2.0**-11)
     half = torch.finfo(dtype).eps / 2
-    top = np.abs(weight).max(axis=-1, keepdims=True) if weight.size else weight
-    out = half * np.abs(ref) * 1.001 + rel[..., None] * weight * 2 + length * 2.0**-25 * top + 1e-30
+    out = half * np.abs(ref) * 1.001 + rel[..., None] * weight * 2 + 2.0**-25 * flush + 1e-30
     le = np.where(np.isfinite(lse), score + 2.0**-20 + length * 2.0**-22 + 2.0**-22 * np.abs(lse), 0.0)
     return out, le

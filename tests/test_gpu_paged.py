@@ -249,6 +249,8 @@ class _Case:
         c = {n: _values(self.pool, n) for n in "kv"}
         s = {n: getattr(self.pool, n + "_scale").double().cpu().numpy() for n in "kv"}
         self.dense = [tuple(P.dense(c[n], s[n], self.table_list[b], m) for n in "kv") for b, m in enumerate(lens)]
+        vs = s["v"]
+        self.vs = [np.repeat(vs[self.table_list[b][: -(-m // page)]], page, axis=0)[:m].T for b, m in enumerate(lens)]  # (H, len)
         self.rng = rng
 
 
@@ -257,8 +259,8 @@ def _check(case, q_rows, out, lse, scaling, dtype, window=0, starts=None):
     worst = 0.0
     for b, (q, o, e) in enumerate(zip(q_rows, out, lse)):
         k, v = case.dense[b]
-        ref, le, weight, size = P.attention(q.double().cpu().numpy(), k, v, scaling, window, 0 if starts is None else starts[b])
-        tol, tol_e = P.bounds(ref, le, weight, size, q.shape[-1], max(1, case.lens_list[b]), dtype)
+        ref, le, *parts = P.attention(q.double().cpu().numpy(), k, v, scaling, window, 0 if starts is None else starts[b], case.vs[b])
+        tol, tol_e = P.bounds(ref, le, *parts, q.shape[-1], max(1, case.lens_list[b]), dtype)
         d = np.abs(o.double().cpu().numpy() - ref)
         assert (d <= tol).all(), (b, float((d / tol).max()))
         g = e.double().cpu().numpy()
@@ -368,8 +370,8 @@ def test_bad_pages_and_lengths_are_skipped_and_reported() -> None:
     assert torch.equal(out[1], good[1]) and bool(out.isfinite().all())
     keep = torch.cat([torch.arange(16), torch.arange(32, 40)]).numpy()
     k, v = (x[:, keep] for x in case.dense[0])
-    ref, _, w, s = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), k, v, 0.125)
-    assert (np.abs(out[0].double().cpu().numpy() - ref) <= P.bounds(ref, ref[..., 0], w, s, 64, 40, torch.float32)[0]).all()
+    ref, le, *parts = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), k, v, 0.125, vs=case.vs[0][:, keep])
+    assert (np.abs(out[0].double().cpu().numpy() - ref) <= P.bounds(ref, le, *parts, 64, 40, torch.float32)[0]).all()
     with pytest.raises(RuntimeError, match="bad indices"):
         case.pool.check_status()
     paged_peek(case.pool, t, case.lens, 40)
@@ -490,8 +492,8 @@ def test_offsets_past_32_bits() -> None:
     q = torch.randn(1, 8, 1, dim, device=DEV, generator=g).to(torch.bfloat16)
     out, lse = paged_attention(pool, table, lens, q, return_lse=True)
     kd, vd = dk[0].double().cpu().numpy(), dv[0].double().cpu().numpy()
-    ref, le, w, s = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), kd, vd, dim**-0.5)
-    tol, _ = P.bounds(ref, le, w, s, dim, 300, torch.bfloat16)
+    ref, le, *parts = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), kd, vd, dim**-0.5)
+    tol, _ = P.bounds(ref, le, *parts, dim, 300, torch.bfloat16)
     assert (np.abs(out[0].double().cpu().numpy() - ref) <= tol).all()
 
 
@@ -524,3 +526,16 @@ def test_refusals_of_calls() -> None:
         paged_peek(case.pool, case.table, case.lens, 4, dtype=torch.float64)
     with pytest.raises(ValueError, match="done must be"):
         PageTables(2, 2, 4, 16, DEV).release(torch.ones(2, device=DEV))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_short_requests_of_a_few_rows(dim) -> None:
+    """Hundreds of units that fill half a pair of row tiles, several to a CTA,
+    beside one that fills both: the row tiles run at their own pace."""
+    lens = [40 + (37 * i) % 300 for i in range(150)]
+    case = _Case("e4m3", dim, 4, 32, lens, seed=12)
+    q_lens = [5] * 150
+    q_lens[75] = 40
+    out = _run(case, q_lens, 4, torch.bfloat16)
+    assert out <= 1.0
+    case.pool.check_status()

@@ -125,7 +125,7 @@ def test_c_call_refusals() -> None:
     assert L.kvd_paged_peek(ref, 2, None, 4, 4, a, 1, v, v, None) != 0
 
     def tables(batch=2, pages=4, page=16, stride=4, num_free=8, capacity=16, lens=a):
-        return L.kvd_page_tables(batch, pages, page, a, a, a, stride, a, num_free, a, capacity, lens, a, a, a, a, None, None)
+        return L.kvd_page_tables(batch, pages, page, a, a, a, stride, a, num_free, a, capacity, lens, a, a, a, a, None, None, 0, None)
 
     for kw, what in ((dict(batch=0), "batch"), (dict(batch=20000), "batch"), (dict(page=8), "page_size"), (dict(stride=2), "stride"),
                      (dict(num_free=-1), "free"), (dict(capacity=-1), "capacity"), (dict(lens=None), "null")):
