@@ -11,7 +11,8 @@ Public surface (drop-in for kvdlra's):
   factored kernel over the compressed cache;
 * :mod:`kvdlra_b200.paged` -- an 8-bit paged cache that holds every token, for
   ragged batches: page tables, the quantising writer, the dense reader and
-  attention over the pages;
+  attention over the pages; :class:`PagedKVCache` is the transformers cache
+  over it;
 * :mod:`kvdlra_b200.harness` -- chunked prefill and greedy decode drivers.
 
 The compute runs in ``_lib/libkvdlra_b200.so`` (built by
@@ -21,6 +22,7 @@ The compute runs in ``_lib/libkvdlra_b200.so`` (built by
 from .cache import BugStreamingCache, BugStreamingLayer, RopeAngles
 from .integrator import augmented_bug_step, blocked_bug_project, blocked_bug_subspace
 from .paged import PagedPool, PageTables, build_page_tables, paged_append, paged_attention, paged_peek
+from .paged_cache import PagedKVCache
 from .press import BUGPress
 from .attention import enable_factored_decode
 
@@ -28,6 +30,6 @@ __all__ = [
     "BugStreamingCache", "BugStreamingLayer", "RopeAngles",
     "augmented_bug_step", "blocked_bug_project", "blocked_bug_subspace", "BUGPress",
     "enable_factored_decode",
-    "PagedPool", "PageTables", "build_page_tables", "paged_append", "paged_attention", "paged_peek",
+    "PagedPool", "PageTables", "build_page_tables", "paged_append", "paged_attention", "paged_peek", "PagedKVCache",
 ]
 __version__ = "0.1.0"

@@ -23,6 +23,10 @@ before.  ``update``'s return contract is unchanged for models that
 do not select the function, so lock-step comparisons against the reference's
 dense peek still hold.
 
+A :class:`kvdlra_b200.PagedKVCache` tags every step, prompts included, and its
+queries are answered from the 8-bit pages (``kvd_paged_attention``: causal, the
+layer's sliding window, the cache's left padding).
+
 An attention module carrying ``kvd_heads = (h0, hc)`` (set by
 :func:`kvdlra_b200.sharding.shard_attention_heads`) answers only the query
 heads of KV heads ``[h0, h0 + hc)``: the factored kernels take the head range,
@@ -61,6 +65,10 @@ def factored_attention_forward(module: torch.nn.Module, query: torch.Tensor, key
                                       scaling=scaling, **kwargs)
     if dropout:
         raise NotImplementedError("factored attention has no dropout (inference only)")
+    if hasattr(layer, "paged_attention"):
+        layer.check_mask(attention_mask, query)
+        window = kwargs.get("sliding_window") or getattr(module, "sliding_window", None) or 0
+        return layer.paged_attention(query, scaling=scaling, heads=heads, window=int(window)), None
     mode = getattr(layer, "_mode", None)
     if mode in ("ingest", "score"):
         # a chunk (or a frozen-scoring window: its own K/V are the tail)

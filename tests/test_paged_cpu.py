@@ -165,3 +165,17 @@ def test_plain_tables_hand_worked() -> None:
 
 def test_module_exports() -> None:
     assert all(hasattr(paged, n) for n in paged.__all__)
+
+
+def test_cache_refusals() -> None:
+    from kvdlra_b200 import PagedKVCache
+
+    for kw, what in ((dict(max_tokens=0), "max_tokens"), (dict(page_size=24), "page_size"), (dict(storage="int4"), "storage"),
+                     (dict(left_padding=torch.tensor([-1])), "left_padding"), (dict(left_padding=torch.zeros(2)), "left_padding")):
+        with pytest.raises(ValueError, match=what):
+            PagedKVCache(None, **{"max_tokens": 8, "num_layers": 1, **kw})
+    cache = PagedKVCache(None, 8, num_layers=2)
+    k = torch.zeros(1, 2, 3, 32)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        cache.update(k, k, 0)
+    assert cache.get_seq_length() == 0 and cache.get_mask_sizes(3, 0) == (3, 0) and cache.stored_state_numel() == 0
