@@ -341,13 +341,28 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       const int id = a.table[(long)p.b * a.table_stride + (tok >> lg)];
       return id < 0 || id >= pool.num_pages ? -2 : id;
     };
-    uint4 raw[4][QC];
-    auto fetch = [&](const Tile& t, int ids) {
+    uint4 raw[4][QC];  // tokens 8 (4k + lw) + tr, block c
+    // Converts what is there to `dst` (unless null) and starts the loads of tile
+    // t, a quarter at a time: a load then has the rest of this tile's conversion
+    // and the wait for a stage to arrive in.
+    auto turn = [&](unsigned char* dst, const Tile& t, int ids) {
       const int sl = max(0, t.sl), lo = pieces[sl].lo, hi = t.sl < 0 ? 0 : pieces[sl].hi;
       const unsigned char* base = codes + (long)pieces[sl].h * pool.head_stride + 16 * cl;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int tg = 4 * k + lw, tok = t.tok0 + 8 * tg + tr;
+        if (dst) {
+#pragma unroll
+          for (int c = 0; c < QC; ++c) {
+            const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) codes_to_f16<STORE>(w[e], &o[2 * e], &o[2 * e + 1]);
+            unsigned char* p = dst + (c ^ (QC - 1 & tr)) * kPcBlock + tg * 1024 + tr * 128;
+            *reinterpret_cast<uint4*>(p + 16 * ((2 * cl) ^ tr)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(p + 16 * ((2 * cl + 1) ^ tr)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
         const int id = __shfl_sync(0xffffffffu, ids, tg >> 1);
         const bool live = id >= 0 && tok >= lo && tok < hi;
         const unsigned char* p = base + (long)id * pool.page_stride + (long)(tok & mask) * pool.slot_stride;
@@ -356,22 +371,6 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (live) asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p + 64 * (c ^ (QC - 1 & tr))));
           raw[k][c] = x;
-        }
-      }
-    };
-    auto put = [&](unsigned char* dst) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int tg = 4 * k + lw;
-#pragma unroll
-        for (int c = 0; c < QC; ++c) {
-          const uint32_t w[4] = {raw[k][c].x, raw[k][c].y, raw[k][c].z, raw[k][c].w};
-          uint32_t o[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) codes_to_f16<STORE>(w[e], &o[2 * e], &o[2 * e + 1]);
-          unsigned char* p = dst + (c ^ (QC - 1 & tr)) * kPcBlock + tg * 1024 + tr * 128;
-          *reinterpret_cast<uint4*>(p + 16 * ((2 * cl) ^ tr)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(p + 16 * ((2 * cl + 1) ^ tr)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
       }
     };
@@ -390,7 +389,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     step(&aft);
     nxt = aft;
     int ids_n = page_id(nxt);
-    fetch(cur, ids);
+    turn(nullptr, cur, ids);
     scale(cur, ids, &ks, &vs);
     for (int it = 0; cur.sl >= 0 && ok; ++it) {
       step(&aft);
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       ok = wait(empty + st, ((it / NS) & 1) ^ 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      put(stages + st * L::tile);
+      turn(stages + st * L::tile, nxt, ids_n);
       if (keys && lw == 0 && lane < 8) {
         ChunkScales& s = scales[it % L::ring];
         s.ks[lane] = ks;
@@ -412,7 +411,6 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       }
       umma::fence_proxy_async_smem();
       umma::mbar_arrive(full + st);
-      fetch(nxt, ids_n);
       if (nxt.sl != cur.sl) umma::mbar_arrive(ne + cur.sl);
       cur = nxt;
       nxt = aft;
@@ -498,6 +496,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           uint32_t s[2][32];
           umma::tmem_ld32(t_b, s[0]);
           umma::tmem_ld32(t_b + 32, s[1]);
+          // meanwhile the scales of the subtile's four 16 tokens
+          const float4 ks4 = *reinterpret_cast<const float4*>(sc.ks + g0), lv4 = *reinterpret_cast<const float4*>(sc.lv + g0);
+          // above zero: a masked -inf stays one
+          const float cg[4] = {fmaxf(ks4.x * cq, 0x1p-126f), fmaxf(ks4.y * cq, 0x1p-126f), fmaxf(ks4.z * cq, 0x1p-126f), fmaxf(ks4.w * cq, 0x1p-126f)};
+          const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
           umma::tmem_wait_ld32(s[0]);
           umma::tmem_loaded32(s[1]);
           if constexpr (decltype(masked)::value) {
@@ -516,9 +519,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
               b1 = max3(b1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
             }
             b0 = max3(b0, __uint_as_float(v[14]), __uint_as_float(v[15]));
-            const float x = fmaxf(b0, b1) * fmaxf(sc.ks[g0 + g] * cq, 0x1p-126f);  // above zero: a masked -inf stays
+            const float x = fmaxf(b0, b1) * cg[g];
             tm = fmaxf(tm, x);
-            tv = fmaxf(tv, x + sc.lv[g0 + g]);
+            tv = fmaxf(tv, x + lv[g]);
           }
           const bool grew = tm > m + kLTop || tv > mv + kPTop;
           if (__any_sync(0xffffffffu, grew)) {
@@ -552,31 +555,27 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           // over a page's tokens, times 2^-d, goes to l
           const float base = m == -INFINITY ? 0.f : -m;
           const float dm = mv == -INFINITY ? 0.f : m - mv;
+          uint32_t p16[32];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p16[16];
+          for (int g = 0; g < 4; ++g) {
+            const float d = fmaxf(lv[g] + dm, -100.f), bg = base + d;
+            const uint64_t c2 = pack2(cg[g], cg[g]), b2 = pack2(bg, bg);
+            uint64_t l2 = pack2(0.f, 0.f);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const int gg = g0 + 2 * c + g;
-              const float cg = fmaxf(sc.ks[gg] * cq, 0x1p-126f);
-              const float d = fmaxf(sc.lv[gg] + dm, -100.f), bg = base + d;
-              const uint64_t c2 = pack2(cg, cg), b2 = pack2(bg, bg);
-              uint64_t l2 = pack2(0.f, 0.f);
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                float x0, x1;
-                unpack2(fma2(pack2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), c2, b2), &x0, &x1);
-                x0 = exp2_fast(x0);
-                x1 = exp2_fast(x1);
-                l2 = add2(l2, pack2(x0, x1));
-                p16[8 * g + e / 2] = pack_f16(x0, x1);
-              }
-              float l0, l1;
-              unpack2(l2, &l0, &l1);
-              l = fmaf(l0 + l1, exp2_fast(-d), l);
+            for (int e = 0; e < 16; e += 2) {
+              float x0, x1;
+              const uint32_t* v = s[g >> 1] + 16 * (g & 1) + e;
+              unpack2(fma2(pack2(__uint_as_float(v[0]), __uint_as_float(v[1])), c2, b2), &x0, &x1);
+              x0 = exp2_fast(x0);
+              x1 = exp2_fast(x1);
+              l2 = add2(l2, pack2(x0, x1));
+              p16[8 * g + e / 2] = pack_f16(x0, x1);
             }
-            umma::tmem_st16(t_b + 16 * c, p16);
+            float l0, l1;
+            unpack2(l2, &l0, &l1);
+            l = fmaf(l0 + l1, exp2_fast(-d), l);
           }
+          umma::tmem_st32(t_b, p16);  // one store: the exponentials of all 64 may overlap
           umma::tmem_wait_st();
           umma::fence_before_sync();
           umma::mbar_arrive(&pf[w][b]);

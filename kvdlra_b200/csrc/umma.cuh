@@ -133,20 +133,18 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) 
 // warp-uniform values are all the arithmetic between them.
 __device__ __forceinline__ void mma_f16_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                               bool accumulate) {
-  const uint32_t z = 0;
   asm volatile(
       "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %5, 0;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, {%6, %6, %6, %6}, p;\n}"
-      ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate), "r"(z)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts_lo(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                               bool accumulate) {
-  const uint32_t z = 0;
   asm volatile(
       "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n mov.b64 db, {%2, %3};\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, {%6, %6, %6, %6}, p;\n}"
-      ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate), "r"(z)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}"
+      ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 

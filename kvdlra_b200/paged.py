@@ -219,10 +219,10 @@ def build_page_tables(cached_lens: Tensor, new_lens: Tensor, table: Tensor, free
     ws = lib.kvd_page_tables_workspace_bytes(batch, capacity)
     n = 2 * cap + 2 * batch + 2
     buf = torch.empty(n + ws // 4, dtype=torch.int32, device=device)
-    slots, positions = buf[:capacity], buf[cap : cap + capacity]
-    cu = buf[2 * cap : 2 * cap + batch + 1]
-    lens = cached_lens if in_place else buf[2 * cap + batch + 1 : 2 * cap + 2 * batch + 1]
-    left = free_count if in_place else buf[n - 1 : n]
+    slots, _, positions, _, cu, lens, left, _ = buf.split_with_sizes(
+        (capacity, cap - capacity, capacity, cap - capacity, batch + 1, batch, 1, ws // 4))
+    if in_place:
+        lens, left = cached_lens, free_count
     _call(device, lib.kvd_page_tables, "kvd_page_tables", batch, table.shape[1], page_size, cached_lens.data_ptr(),
           new_lens.data_ptr(), table.data_ptr(), table.stride(0), free_pages.data_ptr(), free_pages.shape[0],
           free_count.data_ptr(), capacity, lens.data_ptr(), left.data_ptr(), cu.data_ptr(), slots.data_ptr(),
@@ -349,12 +349,12 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     lse = None
     fill = out is None  # rows behind the last request
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q) if packed and q.is_contiguous() else q.new_empty(shape)
     else:
         _need(tuple(out.shape) == shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0,
               f"out must be a contiguous {q.dtype} tensor of shape {shape}, got {out.dtype} {tuple(out.shape)}")
     if return_lse:
-        lse = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+        lse = q.new_empty(shape[:-1], dtype=torch.float32)
         if packed and not fill:
             lse.fill_(-torch.inf)
     ws = torch.empty(pool.workspace_bytes(dtype, hq), dtype=torch.uint8, device=device)
