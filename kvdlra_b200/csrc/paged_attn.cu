@@ -35,6 +35,7 @@
 // takes an equal run of it; a unit that spans CTAs leaves records that
 // paged_merge_kernel joins.  Lengths stay on the device.
 #include <algorithm>
+#include <new>
 
 #include "paged.cuh"
 
@@ -71,7 +72,7 @@ KVD_DEVICE uint32_t transpose_f16x2(uint32_t x) {
 // CTAs of the few-row kernel per SM: as many as its accumulators and the codes
 // in flight leave registers for without spills
 __host__ __device__ constexpr int rows_per_sm(int D, int nt, bool fp32) {
-  return D <= 64 ? (fp32 ? 3 : nt == 1 ? 5 : 4) : D == 128 && nt == 1 && !fp32 ? 3 : 2;
+  return D <= 64 ? (fp32 ? 3 : nt == 1 ? 4 : 3) : D == 128 && nt == 1 && !fp32 ? 3 : 2;
 }
 
 // W words from global memory, read once
@@ -117,10 +118,21 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge waits for this grid's end itself
   const WorkAt at = find_work<RT, TT, kRowThreads>(rq, blockIdx.x, gridDim.x);
-  Pieces<RT, TT> pc(rq, at, blockIdx.x);
-  int4 begun = make_int4(0, 0, 0, 0);
-
-  while (pc.next()) {
+  // The walk over the pieces lies in shared memory and is taken by one thread:
+  // the registers have no room for it beside the codes and the accumulators.
+  __shared__ alignas(16) unsigned char walk[sizeof(Pieces<RT, TT>)];
+  __shared__ int walk_more;
+  __shared__ int4 begun;
+  Pieces<RT, TT>& pc = *reinterpret_cast<Pieces<RT, TT>*>(walk);
+  if (tid == 0) {
+    new (&pc) Pieces<RT, TT>(rq, at, blockIdx.x);
+    begun = make_int4(0, 0, 0, 0);
+  }
+  const long chunk = at.chunk;
+  while (true) {
+    if (tid == 0) walk_more = pc.next();
+    __syncthreads();
+    if (!walk_more) break;
     const int b = pc.b, h = pc.h, row0 = pc.rt * RT, rows = pc.rows, lo = pc.lo, hi = pc.hi;
     const int t_begin = pc.tile * TT, t_end = min(hi, t_begin + pc.n * TT);
     // every row sees [lo_all, hi_all)
@@ -477,8 +489,9 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
         }
       }
     }
-    if (const int n = pc.pieces(at.chunk)) begun = make_int4(b, h, pc.rt, n);
-    __syncthreads();  // the output's readers are done
+    if (tid == 0)
+      if (const int n = pc.pieces(chunk)) begun = make_int4(b, h, pc.rt, n);
+    __syncthreads();  // the output's readers, and the piece's, are done
   }
   if (tid == 0) a.part.head[blockIdx.x] = begun;
 }
