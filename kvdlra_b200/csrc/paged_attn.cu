@@ -108,8 +108,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
   constexpr int RT = Sh::RT, WT = Sh::WT, TT = Sh::TT, KW = Sh::KW, VW = Sh::VW;
   constexpr bool SPLIT = sizeof(T) == 4;
   extern __shared__ __align__(16) float osm[];  // [4 warps][RT][D]
-  __shared__ int seg_id[kSegPages];
-  __shared__ float seg_ks[kSegPages], seg_vs[kSegPages], seg_lv[kSegPages];
+  __shared__ float4 seg[kSegPages];  // of a page: keys' scale, values' scale, log2 of that, id (as bits; < 0: none)
   __shared__ float sm_m[4][RT], sm_l[4][RT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
   const PagedPool& pool = a.pool;
@@ -219,10 +218,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
           id = -1;
         }
         const float vs = id < 0 ? 0.f : pool.vs[(long)id * pool.scale_stride + h];
-        seg_id[i] = id;
-        seg_ks[i] = id < 0 ? 0.f : pool.ks[(long)id * pool.scale_stride + h];
-        seg_vs[i] = vs;
-        seg_lv[i] = log2f(vs);
+        seg[i] = make_float4(id < 0 ? 0.f : pool.ks[(long)id * pool.scale_stride + h], vs, log2f(vs), __int_as_float(id));
       }
       __syncthreads();
 
@@ -232,7 +228,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
           const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
-          const int id = pi < np ? seg_id[pi] : -1;
+          const int id = pi < np ? __float_as_int(seg[pi].w) : -1;
           const unsigned char* p = pool.k + (long)id * pool.page_stride + (long)h * pool.head_stride +
                                    (long)((tb & page_mask) + g) * pool.slot_stride + (D == 32 ? 8 : 16) * j;
 #pragma unroll
@@ -252,7 +248,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
           const int tb = t + 16 * s, pi = (tb >> lg) - pg0;
-          const int id = pi < np ? seg_id[pi] : -1;
+          const int id = pi < np ? __float_as_int(seg[pi].w) : -1;
           const unsigned char* p = pool.v + (long)id * pool.page_stride + (long)h * pool.head_stride +
                                    (long)((tb & page_mask) + 2 * j) * pool.slot_stride + (D / 8) * g;
 #pragma unroll
@@ -301,11 +297,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
         bool bad[ST];
 #pragma unroll
         for (int u = 0; u < ST; ++u) {
-          const int pi = min(((t + 16 * u) >> lg) - pg0, np - 1);
-          ksc[u] = seg_ks[pi];
-          vsc[u] = seg_vs[pi];
-          lvs[u] = seg_lv[pi];
-          bad[u] = ((t + 16 * u) >> lg) - pg0 >= np || seg_id[pi] < 0;
+          const int pi = ((t + 16 * u) >> lg) - pg0;
+          const float4 e = seg[min(pi, np - 1)];
+          ksc[u] = e.x;
+          vsc[u] = e.y;
+          lvs[u] = e.z;
+          bad[u] = pi >= np || __float_as_int(e.w) < 0;
           whole = whole && !bad[u];
         }
         if (t + TT < t_seg1) key_words(t + TT, kw);
@@ -539,9 +536,12 @@ int paged_pool_view(const kvd_paged_pool* p, PagedPool* out) {
 // read once per 8 or 16 rows, the tensor-memory kernel's once per 256.
 constexpr int kFewRows = 16;
 
-// rows per unit of the few-row kernel: eight, or sixteen for longer groups
-// (head_dim 256: sixteen rows' accumulators would not fit the registers)
+// Rows of a unit / 8: one, or two where a request has more than eight rows
+// (head_dim 256: sixteen rows' accumulators would not fit the registers; thirty-two
+// rows at head_dim 64 fit, but took 237 us where sixteen take 211, for 24 fp32
+// requests of 1 to 257 rows).
 static int rows_nt(long max_rows, int D) { return max_rows <= 8 || D == 256 ? 1 : 2; }
+// CTAs that fit an SM (the kernel's launch bounds)
 static int rows_ctas(int D, int nt, bool fp32) { return paged_sm_count() * rows_per_sm(D, nt, fp32); }
 
 template <int D, int NT, int STORE, typename T>
