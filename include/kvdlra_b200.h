@@ -336,7 +336,8 @@ int kvd_paged_peek(const kvd_paged_pool* pool, int32_t batch, const int32_t* tab
 /* Attention over the pages.  Request b's queries are its last tokens: query i
  * of its n sees tokens t <= lens[b] - n + i, t >= starts[b] (left padding;
  * starts may be NULL) and, with window > 0, t > lens[b] - n + i - window.  A
- * row that sees nothing gives zeros and lse -inf.  cu_q [batch + 1] (packed
+ * row that sees nothing gives zeros and lse -inf.  Lengths are held to
+ * max_pages * page_size; codes are finite (kvd_paged_append writes no others).  cu_q [batch + 1] (packed
  * queries, q_tokens rows in all, max_q the most of one request or 0 for not
  * known) or NULL (every request has q_tokens).  scaling > 0; scales > 0 or 0.  q: element strides of batch,
  * head and token, multiples of 16 bytes, unit stride over D.  out

@@ -619,7 +619,8 @@ extern "C" int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, co
     return KVD_ERR_WORKSPACE;
   }
   PagedReqs& r = a.reqs;
-  r.batch = batch; r.H = H; r.G = G; r.q_tokens = q_tokens; r.window = window;
+  r.batch = batch; r.H = H; r.G = G; r.q_tokens = q_tokens;
+  r.window = std::min(window, 1 << 30);  // more than any request holds: place and window stay within 32 bits
   r.max_len = max_pages * pool->page_size;
   r.lens = lens; r.cu_q = cu_q; r.starts = starts;
   r.min_rows = 1; r.max_rows = INT32_MAX;

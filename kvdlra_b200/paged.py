@@ -303,6 +303,9 @@ def paged_peek(pool: PagedPool, table: Tensor, lens: Tensor, tokens: int, *, dty
     _need(tokens >= 0, f"tokens must be >= 0, got {tokens}")
     kv = torch.empty((2, batch, pool.num_heads, tokens, pool.head_dim), dtype=dtype, device=pool.device)
     k, v = kv.unbind(0)
+    if table.shape[1] == 0:
+        kv.zero_()
+        return k, v
     _call(pool.device, N.lib().kvd_paged_peek, "kvd_paged_peek", pool._ref, batch, table.data_ptr(), table.stride(0), table.shape[1],
           lens.data_ptr(), code, _view(k), _view(v), _stream(pool.device.index))
     return k, v
@@ -319,7 +322,10 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     sees tokens up to ``lens[b] - n + i``, from ``starts[b]`` on (left padding)
     and, with ``window > 0``, only the last ``window`` of them.  A query that
     sees nothing gives zeros.  ``max_q``: the most query tokens of one packed
-    request, if known; it only chooses kernels.
+    request, if known; it only chooses kernels.  ``scaling`` is positive, ``D ** -0.5``
+    if not given.  Lengths beyond the table's columns end with them; ``cu_q``
+    entries that are no offsets into the rows answer nothing.  The pages' codes are
+    finite, as :func:`paged_append` writes them.
 
     Returns ``(B, T, Hq, D)``, or ``(rows, Hq, D)`` packed, in ``q``'s type
     (rows behind ``cu_q[B]`` are zero, or as they were in ``out``), and with
@@ -351,12 +357,19 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     if out is None:
         out = torch.empty_like(q) if packed and q.is_contiguous() else q.new_empty(shape)
     else:
-        _need(tuple(out.shape) == shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0,
-              f"out must be a contiguous {q.dtype} tensor of shape {shape}, got {out.dtype} {tuple(out.shape)}")
+        _need(tuple(out.shape) == shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0
+              and out.untyped_storage().data_ptr() != q.untyped_storage().data_ptr(),
+              f"out must be a contiguous {q.dtype} tensor of shape {shape} with memory of its own, got {out.dtype} {tuple(out.shape)}")
     if return_lse:
         lse = q.new_empty(shape[:-1], dtype=torch.float32)
         if packed and not fill:
             lse.fill_(-torch.inf)
+    if batch == 0 or table.shape[1] == 0:  # nobody has tokens
+        if fill or not packed:
+            out.zero_()
+        if lse is not None:
+            lse.fill_(-torch.inf)
+        return out if lse is None else (out, lse)
     ws = torch.empty(pool.workspace_bytes(dtype, hq), dtype=torch.uint8, device=device)
     view = _view(q)
     _call(device, N.lib().kvd_paged_attention, "kvd_paged_attention", pool._ref, batch, table.data_ptr(), table.stride(0), table.shape[1],

@@ -539,3 +539,91 @@ def test_many_short_requests_of_a_few_rows(dim) -> None:
     out = _run(case, q_lens, 4, torch.bfloat16)
     assert out <= 1.0
     case.pool.check_status()
+
+
+@pytest.mark.parametrize("dim, order, dtype", [(64, "pshd", torch.bfloat16), (128, "pshd", torch.float16), (128, "phsd", torch.bfloat16)])
+def test_chunks_of_strided_pools_and_queries(dim, order, dtype) -> None:
+    """Many rows over page-slot-head pools, a range of KV heads, (B, Hq, T, D)
+    queries as a projection leaves them, lengths at the tiles' borders."""
+    case = _Case("int8", dim, 3, 32, [127, 300, 128, 64], seed=14, order=order)
+    base = torch.tensor(case.rng.standard_normal((4, 61, 8, dim)), dtype=dtype, device=DEV)  # (B, T, heads, D)
+    q = base.transpose(1, 2)[:, 1:7]
+    out, lse = paged_attention(case.pool, case.table, case.lens, q, return_lse=True)
+    _check(case, [q[b].transpose(0, 1) for b in range(4)], out, lse, dim**-0.5, dtype)
+    part = paged_attention(case.pool.heads(1, 2), case.table, case.lens, q[:, 2:])
+    assert float((part.double() - out[:, :, 2:].double()).abs().max()) <= 2.0**-7 * float(out.double().abs().max())  # other units, other splits
+    case.pool.check_status()
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_a_window_beyond_every_length_hides_nothing(n) -> None:
+    case = _Case("e4m3", 64, 1, 16, [40, 3], seed=15)
+    q = torch.randn(2, 2, n, 64, device=DEV).to(torch.bfloat16)
+    plain = paged_attention(case.pool, case.table, case.lens, q)
+    for window in (40, 2**31 - 1):
+        assert torch.equal(paged_attention(case.pool, case.table, case.lens, q, window=window), plain)
+
+
+def test_scales_of_another_size_and_zero() -> None:
+    """Attention and peek take any scales: values' scales 2^60 apart, one of 0."""
+    for n in (1, 24):
+        case = _Case("int8", 64, 1, 16, [64, 50], seed=16)
+        ids = case.table_list[0]
+        case.pool.v_scale[ids[0]] *= 2.0**30
+        case.pool.v_scale[ids[2]] *= 2.0**-30
+        case.pool.v_scale[ids[1]] = 0
+        case.pool.k_scale[ids[3]] = 0
+        s = {x: getattr(case.pool, x + "_scale").double().cpu().numpy() for x in "kv"}
+        case.dense = [tuple(P.dense(_values(case.pool, x), s[x], case.table_list[b], m) for x in "kv") for b, m in enumerate(case.lens_list)]
+        vs = np.repeat(s["v"][ids[:4]], 16, axis=0).T
+        case.vs[0] = np.where(vs == 0, 2.0**-20, vs)  # a scale of 0: values of 0, whatever it counts as
+        _run(case, [n, n], 4, torch.bfloat16)
+
+
+def test_nothing_to_do() -> None:
+    pool = PagedPool.allocate(4, 16, 2, 64, device=DEV)
+    none = torch.empty((0, 3), dtype=torch.int32, device=DEV)
+    q = torch.randn(5, 4, 64, device=DEV)
+    out, lse = paged_attention(pool, none, _i32([]), q, cu_q=_i32([0]), return_lse=True)
+    assert not out.any() and bool((lse == -torch.inf).all())
+    empty = torch.empty((2, 0), dtype=torch.int32, device=DEV)
+    out = paged_attention(pool, empty, _i32([0, 0]), q[:2, :, None])
+    assert out.shape == (2, 1, 4, 64) and not out.any()
+    assert not paged_peek(pool, empty, _i32([0, 0]), 3)[0].any()
+    assert paged_peek(pool, empty, _i32([0, 0]), 0)[1].shape == (2, 2, 0, 64)
+    assert paged_attention(pool, _i32([[0]]), _i32([1]), q[:0], cu_q=_i32([0, 0])).shape == (0, 4, 64)
+    p = build_page_tables(_i32([0, 3]), _i32([0, 0]), _i32([[-1], [2]]), _i32([]), _i32([0]), page_size=16, capacity=0)
+    assert p.cu_new.tolist() == [0, 0, 0] and p.lens.tolist() == [0, 3] and p.free_count.item() == 0
+
+
+def test_more_refusals() -> None:
+    case = _Case("int8", 64, 2, 16, [20], seed=0)
+    q = torch.randn(1, 4, 1, 64, device=DEV)
+    for scaling in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(RuntimeError, match="scaling"):
+            paged_attention(case.pool, case.table, case.lens, q, scaling=scaling)
+    with pytest.raises(ValueError, match="memory of its own"):
+        paged_attention(case.pool, case.table, case.lens, q, out=q.view(1, 1, 4, 64))
+
+
+def test_a_captured_call_and_an_eager_one_side_by_side() -> None:
+    """Two graphs and an eager call of one pool, on three streams at once."""
+    case = _Case("e4m3", 64, 2, 16, [2000, 900], seed=17)
+    qs = [torch.randn(2, 8, n, 64, device=DEV).to(torch.bfloat16) for n in (1, 40, 1)]
+    want = [paged_attention(case.pool, case.table, case.lens, q) for q in qs]
+    graphs, outs = [], []
+    for q in qs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention(case.pool, case.table, case.lens, q))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = paged_attention(case.pool, case.table, case.lens, qs[2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs + [eager], want))
