@@ -5,17 +5,20 @@
 // (request, KV head, 256 query rows), a row (token, head of the group).  Per
 // 128-token tile:
 //   loaders (4 warps for keys, 4 for values)  the page's codes from global
-//                      memory, a tile ahead in registers, converted exactly to f16 and written to shared
-//                      memory as rows of 64 dims with the 128-byte swizzle: the
-//                      same image is a K-major operand of the scores and an
-//                      MN-major one of the values.
-//   issuer (1 thread)  S_w = Q_w K^T for the two row tiles w of 128 rows, and
-//                      O_w += P_w V with P_w in TMEM; while one row tile's
-//                      softmax runs, the tensor core works for the other.
+//                      memory, a tile ahead in registers, converted exactly to
+//                      f16 and written to shared memory as rows of 64 dims with
+//                      the 128-byte swizzle: the same image is a K-major operand
+//                      of the scores and an MN-major one of the values.
+//   issuer (1 warp)    S_w = Q_w K^T for the two row tiles w of 128 rows, and
+//                      O_w += P_w V with P_w in TMEM, by subtiles of 64 tokens.
+//                      S has two buffers per row tile: the next scores are there
+//                      while this subtile's weights are computed.
 //   softmax (2 x 4 warps)  a thread owns a row (a TMEM lane): the row's maxima
-//                      and sums need no other thread.  P_w (f16) goes over the
-//                      columns of S_w.
-// TMEM: S_0, S_1 (128 columns each), O_0, O_1 (head_dim each).
+//                      and sums need no other thread.  S is read once, in one wait
+//                      (TMEM reads are slow beside the tensor core); P_w (f16) goes
+//                      over the columns of S_w.
+//   planner (1 thread) the walk over the requests, handed on piece by piece.
+// TMEM: S_0, S_1 (two buffers of 64 columns each), O_0, O_1 (head_dim each).
 //
 // Two references per row, in base 2: m for the sum l of the weights, and mv
 // for O, whose weights carry the page's value scale: p vs = 2^(x - m) (vs 2^(m -
@@ -27,9 +30,14 @@
 // elements 2^-13 of the row's largest); S, O, m, l are fp32; P is rounded to
 // f16 (2^-11).
 //
-// Bound, per tile of 256 rows x 128 tokens at head_dim 128 and clock: tensor
-// core 2048, exponentials 2048 (16 a clock), shared memory about 2048 (Q, K and
-// V operands, and the converted tiles).
+// Bound, per tile of 256 rows x 128 tokens at head_dim 128, in clocks: tensor
+// core 2048, exponentials 2176 (8 a warp), shared memory 2500 (Q and K once per
+// subtile, V, the converted tiles).  Measured: 4900, 1.3 ms and 818 TFLOP/s for
+// 2048 queries of 32768 tokens with 32 heads over 8 (int8 pages, bf16).  S of 128
+// tokens in one buffer (fewer reads of Q, the softmax waits for it) took as long;
+// the exponentials' share, or the count of the softmax's instructions, made no
+// difference.  Loaders of one warpgroup, and 16 softmax warps with half a row each,
+// ran out of registers.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -655,6 +663,15 @@ template <int D, int STORE, typename T>
 static int launch_chunk(ChunkArgs& a, int fill_tail, void* ws, cudaStream_t s) {
   auto kern = paged_chunk_kernel<D, STORE, T>;
   if (int rc = ensure_smem((const void*)kern, ChunkSmem<D>::total, "paged_chunk_kernel")) return rc;
+  // The warpgroups' shares draw on what the CTA is launched with: fewer registers,
+  // from another compiler, and they would wait for good.
+  static int regs = 0;
+  if (!regs) {
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, (const void*)kern) != cudaSuccess) { set_error("paged_chunk_kernel: no attributes"); return KVD_ERR_CUDA; }
+    regs = attr.numRegs;
+  }
+  if (regs != kPcRegsLaunch) { set_error("paged_chunk_kernel was built with %d registers, not %d", regs, kPcRegsLaunch); return KVD_ERR_CUDA; }
   const int ctas = paged_sm_count();
   a.part = part_at(ws, ctas);
   {

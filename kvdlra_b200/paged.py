@@ -89,26 +89,24 @@ def _cuda(device: torch.device) -> None:
         raise RuntimeError(f"kvdlra_b200.paged runs on CUDA devices only (no CPU fallback); got a tensor on {device}")
 
 
-def _no_grad(*ts: Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+def _no_grad(a: Tensor, b: Tensor | None = None) -> None:
+    if (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("the 8-bit paged cache is inference only: call it under torch.no_grad()")
 
 
-def _rows(t: Tensor) -> Tensor:
-    """``t`` with a contiguous, 16-byte-aligned last dimension."""
-    n = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % n for s, m in zip(t.stride()[:-1], t.shape) if m > 1):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _view(t: Tensor) -> N.HFView:
-    """The C view of ``(B, H, T, D)`` (or packed ``(T, H, D)``); strides of
-    dimensions of one element, which are never used, as 0."""
-    st, sh = t.stride(), t.shape
-    if t.dim() == 3:
-        return N.HFView(t.data_ptr(), 0, st[1] if sh[1] > 1 else 0, st[0] if sh[0] > 1 else 0, sh[0])
-    return N.HFView(t.data_ptr(), st[0] if sh[0] > 1 else 0, st[1] if sh[1] > 1 else 0, st[2] if sh[2] > 1 else 0, sh[2])
+def _rows(t: Tensor) -> tuple[Tensor, N.HFView]:
+    """``t`` ``(B, H, T, D)`` or packed ``(T, H, D)`` with a contiguous,
+    16-byte-aligned last dimension (a copy where it has none), and its C view.
+    Strides of dimensions of one element, which are never used, count as 0."""
+    st, sh, n = t.stride(), t.shape, 16 // t.element_size()
+    if len(sh) == 3:
+        tokens, sb, hs, ts = sh[0], 0, st[1] if sh[1] > 1 else 0, st[0] if sh[0] > 1 else 0
+    else:
+        tokens, sb, hs, ts = sh[2], st[0] if sh[0] > 1 else 0, st[1] if sh[1] > 1 else 0, st[2] if sh[2] > 1 else 0
+    ptr = t.data_ptr()
+    if st[-1] != 1 or ptr % 16 or sb % n or hs % n or ts % n:
+        return _rows(t.clone(memory_format=torch.contiguous_format))
+    return t, N.HFView(ptr, sb, hs, ts, tokens)
 
 
 class PagedPool:
@@ -286,8 +284,9 @@ def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor) -> None:
     _need(k.device == pool.device and v.device == pool.device, f"k and v must be on {pool.device}")
     _ints(slots, (batch * tokens,), "slots", pool.device)
     _no_grad(k, v)
-    k, v = _rows(k), _rows(v)
-    _call(pool.device, N.lib().kvd_paged_append, "kvd_paged_append", pool._ref, slots.data_ptr(), batch, dtype, _view(k), _view(v),
+    k, k_view = _rows(k)  # the copies, if any, live until the call is made: the allocator orders their reuse by stream
+    v, v_view = _rows(v)
+    _call(pool.device, N.lib().kvd_paged_append, "kvd_paged_append", pool._ref, slots.data_ptr(), batch, dtype, k_view, v_view,
           _stream(pool.device.index))
 
 
@@ -307,7 +306,7 @@ def paged_peek(pool: PagedPool, table: Tensor, lens: Tensor, tokens: int, *, dty
         kv.zero_()
         return k, v
     _call(pool.device, N.lib().kvd_paged_peek, "kvd_paged_peek", pool._ref, batch, table.data_ptr(), table.stride(0), table.shape[1],
-          lens.data_ptr(), code, _view(k), _view(v), _stream(pool.device.index))
+          lens.data_ptr(), code, _rows(k)[1], _rows(v)[1], _stream(pool.device.index))
     return k, v
 
 
@@ -351,7 +350,7 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     if starts is not None:
         _ints(starts, (batch,), "starts", device)
     _no_grad(q)
-    q = _rows(q)
+    q, view = _rows(q)
     lse = None
     fill = out is None  # rows behind the last request
     if out is None:
@@ -371,7 +370,6 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
             lse.fill_(-torch.inf)
         return out if lse is None else (out, lse)
     ws = torch.empty(pool.workspace_bytes(dtype, hq), dtype=torch.uint8, device=device)
-    view = _view(q)
     _call(device, N.lib().kvd_paged_attention, "kvd_paged_attention", pool._ref, batch, table.data_ptr(), table.stride(0), table.shape[1],
           lens.data_ptr(), None if starts is None else starts.data_ptr(), None if cu_q is None else cu_q.data_ptr(), dtype,
           view.ptr, view.stride_b, view.stride_h, view.stride_t, tokens, max_q, hq, dim**-0.5 if scaling is None else scaling, window,
