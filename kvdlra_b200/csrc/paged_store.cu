@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
   constexpr int PER = (2048 * (int)sizeof(T)) / 512;  // loads per thread of a whole page: 8 or 16
   __shared__ int slot_sm[2 * kMaxPage + 1];
   __shared__ uint32_t brk[2 * kMaxPage / 32];     // row i does not continue row i - 1's run
-  __shared__ float red[NTHR / 32];
+  __shared__ float red[2][NTHR / 32];             // of every other reduction, so that one barrier does for each
   const PagedPool& pool = a.pool;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = tid / GT, gt = tid % GT;
@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
   __syncthreads();
   unsigned char* codes = kv ? pool.v : pool.k;
   float* scales = kv ? pool.vs : pool.ks;
+  int turn = 0;
   for (int i0 = 0; i0 < a.per_cta; ) {
     // the next run that begins at or after row i0 (and its end)
     int i = i0;
@@ -98,16 +99,20 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
     n = min(n, (mask + 1) - (slot & mask));
     const int page = slot >> lg, o = slot & mask;
     unsigned char* base = codes + (long)page * pool.page_stride + (long)h * pool.head_stride;
+    float* sp = scales + (long)page * pool.scale_stride + h;
+    const float was = live_head && o > 0 ? *sp : 0.f;  // read before the barriers that stand before its write
     // ---- the run's rows, and their largest finite magnitude
     uint4 x[PER];
+    const int b0 = (int)(r0 + i) / a.tokens, t0 = (int)(r0 + i) - b0 * a.tokens;  // one division a run
     float amax = 0.f, odd = 0.f;  // odd: 0, or NaN once a value is not finite
 #pragma unroll
     for (int c = 0; c < PER; ++c) {
       const int e = gt + c * GT, row = e / CPR;
       x[c] = make_uint4(0u, 0u, 0u, 0u);
       if (live_head && row < n) {
-        const long r = r0 + i + row, bt = r / a.tokens;
-        const T* src = reinterpret_cast<const T*>(a.x[kv]) + bt * a.sb[kv] + (long)h * a.sh[kv] + (r - bt * a.tokens) * a.st[kv];
+        int bt = b0, t = t0 + row;
+        while (t >= a.tokens) { t -= a.tokens; ++bt; }
+        const T* src = reinterpret_cast<const T*>(a.x[kv]) + (long)bt * a.sb[kv] + (long)h * a.sh[kv] + (long)t * a.st[kv];
         x[c] = *reinterpret_cast<const uint4*>(src + (e % CPR) * VE);
       }
     }
@@ -124,34 +129,19 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
     auto group_max = [&](float v) {
       v = warp_max(v);
       if constexpr (W > 1) {
-        if (lane == 0) red[warp] = v;
+        turn ^= 1;
+        if (lane == 0) red[turn][warp] = v;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) v = fmaxf(v, red[group * W + w]);
-        __syncthreads();
+        for (int w = 0; w < W; ++w) v = fmaxf(v, red[turn][group * W + w]);
       }
       return v;
     };
     // one number tells both: +inf where a value is not finite
     amax = group_max(odd == 0.f ? amax : INFINITY);
-    if constexpr (W > 1) {
-      // groups of a CTA decide together, for the barriers below
-      if (__syncthreads_or(amax == INFINITY)) {
-        float fin = 0.f;
-#pragma unroll
-        for (int c = 0; c < PER; ++c) {
-          const T* v = reinterpret_cast<const T*>(&x[c]);
-#pragma unroll
-          for (int q = 0; q < VE; ++q) {
-            const float f = fabsf(load_f(v + q));
-            if (f < INFINITY) fin = fmaxf(fin, f);
-          }
-        }
-        const bool flagged = amax == INFINITY;
-        amax = group_max(fin);
-        if (flagged && gt == 0) pool.flag(kStatusNumeric, kPagedNonFinite);
-      }
-    } else if (amax == INFINITY) {
+    bool again = amax == INFINITY;
+    if constexpr (W > 1 && GROUPS > 1) again = __syncthreads_or(again);  // the groups of a CTA meet at the barriers
+    if (again) {
       float fin = 0.f;
 #pragma unroll
       for (int c = 0; c < PER; ++c) {
@@ -162,13 +152,10 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
           if (f < INFINITY) fin = fmaxf(fin, f);
         }
       }
+      if (amax == INFINITY && gt == 0) pool.flag(kStatusNumeric, kPagedNonFinite);
       amax = group_max(fin);
-      if (gt == 0) pool.flag(kStatusNumeric, kPagedNonFinite);
     }
     float s = code_scale<STORE>(amax);
-    float* sp = scales + (long)page * pool.scale_stride + h;
-    const float was = live_head && o > 0 ? *sp : 0.f;
-    if constexpr (W > 1) __syncthreads();  // read by all before it is written
     const bool grew = o > 0 && s > was;
     s = o > 0 ? fmaxf(s, was) : s;
     if (!live_head) continue;
