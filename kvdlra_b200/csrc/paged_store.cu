@@ -30,6 +30,7 @@ struct AppendArgs {
   const void* x[2];    // keys, values
   long sb[2], sh[2], st[2];  // strides of batch, head, token (elements)
   int per_cta;         // consecutive rows whose runs one CTA takes
+  int head_groups;     // CTAs that share the heads
 };
 
 constexpr int kMaxPage = 128;
@@ -48,10 +49,11 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
   const PagedPool& pool = a.pool;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = tid / GT, gt = tid % GT;
-  const int h = blockIdx.y * GROUPS + group, kv = blockIdx.z;
+  // neighbouring CTAs take neighbouring heads of the same rows, which lie together
+  const int h = (int)(blockIdx.x % a.head_groups) * GROUPS + group, kv = blockIdx.y;
   const bool live_head = h < pool.H;
   const int lg = pool.lg_page, mask = pool.page() - 1;
-  const long r0 = (long)blockIdx.x * a.per_cta;
+  const long r0 = (long)(blockIdx.x / a.head_groups) * a.per_cta;
   const int span = a.per_cta + pool.page();       // a run of this CTA ends within it
   const int limit = pool.num_pages << lg;
   for (int i = tid; i <= span; i += NTHR) {
@@ -286,7 +288,10 @@ static int launch_append(AppendArgs& a, cudaStream_t s) {
   // (single tokens are runs of their own: one per CTA spreads them)
   a.per_cta = page;
   while (a.per_cta > 1 && (a.rows + a.per_cta - 1) / a.per_cta * hy * 2 < 2L * paged_sm_count()) a.per_cta >>= 1;
-  const dim3 grid((unsigned)((a.rows + a.per_cta - 1) / a.per_cta), hy, 2);
+  a.head_groups = hy;
+  const long ctas = (a.rows + a.per_cta - 1) / a.per_cta * hy;
+  if (ctas > INT32_MAX) { set_error("paged append: %ld rows of %d heads", a.rows, a.pool.H); return KVD_ERR_ARG; }
+  const dim3 grid((unsigned)ctas, 2);
   KTimerScope kts_("paged_append_kernel", s);
 #define KVD_APPEND(w) \
   case w: paged_append_kernel<D, w, STORE, T><<<grid, w < 4 ? 128 : 32 * w, 0, s>>>(a); break;
