@@ -5,6 +5,8 @@
 // for the keys and for the values, and one fp32 scale each: x = code * scale.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"
@@ -300,16 +302,16 @@ struct PagedOut {
 // 2^(m_i - M) l_i.  blockIdx.x is the CTA of the kernel before that began the
 // unit (most began none that others finish); the rows go over blockIdx.y and the
 // warps.  A row is a warp's, or the four warps' where there are many records (a
-// long context split over the SMs): the lanes find the records' factors, one
+// long context split over the SMs): the lanes find the records' factors, two
 // each, then every lane sums its columns over them.  Bound by the latency of a
-// few dependent reads: 4 us for 64 records, where one pass for the maximum and one
-// for the sums, a thread per column, took 41.
+// few dependent reads: the head, the maxima and sums, the records.
 template <int D, int RT, typename T>
 __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPart part, PagedOut out, int fill_tail) {
   constexpr int V = D < 128 ? D / 32 : 4;      // columns per lane and step
   constexpr int C = D / (32 * V);              // steps
   __shared__ float sums[4][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 u = part.head[blockIdx.x];
   if (fill_tail && rq.cu_q) {  // rows behind the last request: zeros
     const long from = (long)max(0, min(rq.cu_q[rq.batch], rq.q_tokens)) * out.Hq, to = (long)rq.q_tokens * out.Hq;
     const long stride = (long)gridDim.x * gridDim.y * 128;
@@ -318,7 +320,6 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPar
     if (out.lse)
       for (long e = from + at; e < to; e += stride) out.lse[e] = -INFINITY;
   }
-  const int4 u = part.head[blockIdx.x];
   if (u.w == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = u.x, h = u.y, rt = u.z, n = u.w;
@@ -331,25 +332,37 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPar
   const bool many = n >= 12;
   const int per = many ? 1 : 4, stride = many ? 4 : 1, part0 = many ? warp : 0;
   for (int r = blockIdx.y * per + (many ? 0 : warp); r < rows; r += gridDim.y * per) {
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, record(i)[RT * D + r]);
-    M = warp_max(M);
-    float L = 0.f, o[C][V];
+    float M = -INFINITY, L = 0.f, o[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int k = 0; k < V; ++k) o[c][k] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      float f = 0.f;
-      if (i0 + lane < n) {
-        const float* p = record(i0 + lane);
-        f = M == -INFINITY ? 1.f : exp2_fast(p[RT * D + r] - M);
-        L = fmaf(f, p[RT * D + RT + r], L);
+    for (int i0 = 0; i0 < n; i0 += 64) {  // two records a lane
+      float m2[2], l2[2], f2[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = i0 + 32 * k + lane;
+        const float* p = record(min(i, n - 1)) + RT * D + r;
+        m2[k] = i < n ? p[0] : -INFINITY;
+        l2[k] = i < n ? p[RT] : 0.f;
       }
-      const int m = min(32, n - i0);
-#pragma unroll 4
+      const float top = fmaxf(M, warp_max(fmaxf(m2[0], m2[1])));
+      const float old = M == -INFINITY ? 1.f : exp2_fast(M - top);
+      M = top;
+      L *= old;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f2[k] = M == -INFINITY ? 1.f : exp2_fast(m2[k] - M);
+        L = fmaf(f2[k], l2[k], L);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[c][k] *= old;
+      const int m = min(64, n - i0);
+#pragma unroll 8
       for (int i = part0; i < m; i += stride) {
-        const float w = __shfl_sync(0xffffffffu, f, i);
+        const float w = __shfl_sync(0xffffffffu, i < 32 ? f2[0] : f2[1], i & 31);
         const float* p = record(i0 + i) + r * D + V * lane;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -428,7 +441,8 @@ int launch_merge(const PagedReqs& rq, const PagedPart& part, const PagedOut& out
                         cudaStream_t s) {
   // starts while the kernel before it drains, and waits for it in the kernel
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, RT < 32 ? RT : 32);
+  const long rows = std::min((long)RT, (long)rq.q_tokens * rq.G);
+  cfg.gridDim = dim3(ctas, (unsigned)std::min(32L, rows));
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
