@@ -31,6 +31,11 @@
 // the running maxima only when these pass them by kLTop and kPTop: a tile costs
 // one vote instead of reductions over the lanes.
 //
+// Measured: 64 requests of 1 to 32768 tokens, 32 heads over 8 of 128, int8: 419 us,
+// 5.1 TB/s, 79 % of the copy rate; one of 131072 tokens, e4m3: 61 us, 4.4 TB/s.  The
+// conversions' and the softmax's instructions bound it (half of all issue slots at
+// three warps a scheduler): a prefetch of the tile after next into L2 gained nothing.
+//
 // Work: (request, KV head, row tile, 128-token tile) is one list, every CTA
 // takes an equal run of it; a unit that spans CTAs leaves records that
 // paged_merge_kernel joins.  Lengths stay on the device.
@@ -533,7 +538,9 @@ int paged_pool_view(const kvd_paged_pool* p, PagedPool* out) {
 }
 
 // A request of at most this many rows goes to the few-row kernel: its codes are
-// read once per 8 or 16 rows, the tensor-memory kernel's once per 256.
+// read once per 8 or 16 rows, the tensor-memory kernel's once per 256.  At 32 rows
+// (96 requests of 4 drafted tokens, head_dim 128) the first takes 203 us, the other
+// 190.
 constexpr int kFewRows = 16;
 
 // Rows of a unit / 8: one, or two where a request has more than eight rows

@@ -20,8 +20,9 @@ namespace kvd {
 // A group of W warps takes a (run, head, keys or values) item: the run's rows
 // are read once, 16 bytes a load, and stay in registers between the maximum
 // and the codes (W = page * D / 2048 warps hold a whole page in 8 or 16
-// registers a lane).  HBM bounds it for prompts (reads 2 or 4 bytes and writes
-// one per value), latency for single tokens.
+// registers a lane).  A prompt's floor is HBM's (2 or 4 bytes read and one written
+// per value); four prompts of 8191 tokens, 8 heads of 128, take 69 us where that is
+// 31: a CTA's reads wait in turn for its slots.  Single tokens are latency, 3.5 us.
 struct AppendArgs {
   PagedPool pool;
   const int* slots;
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
 // Dense keys and values of requests, (B, H, T, D) in the model's type: row t
 // is code * scale, zero from the request's length on.  One 16-byte store per
 // thread and step, neighbouring threads on neighbouring bytes.  HBM bounds it:
-// one byte read and 2 or 4 written per value.
+// one byte read and 2 or 4 written per value (four prompts of 8191 tokens, 8 heads
+// of 128, to f16: 32 us, 6.3 TB/s).
 struct PeekArgs {
   PagedPool pool;
   const int* table;
@@ -284,10 +286,12 @@ static int launch_append(AppendArgs& a, cudaStream_t s) {
   const int W = std::max(1, page * D / 2048);
   const int groups = W < 4 ? 4 / W : 1;
   const int hy = (a.pool.H + groups - 1) / groups;
-  // a page's worth of rows per CTA, fewer while the grid would leave SMs idle
-  // (single tokens are runs of their own: one per CTA spreads them)
+  // A page's worth of rows per CTA, fewer while the grid would leave most SMs
+  // idle: single tokens are runs of their own and are taken one after another (32
+  // of them, 8 heads of 64: 3.5 us at one per CTA, 28 at sixteen); a chunk of 512
+  // rows is better left whole (4.9 us; 6.0 at four rows per CTA).
   a.per_cta = page;
-  while (a.per_cta > 1 && (a.rows + a.per_cta - 1) / a.per_cta * hy * 2 < 2L * paged_sm_count()) a.per_cta >>= 1;
+  while (a.per_cta > 1 && (a.rows + a.per_cta - 1) / a.per_cta * hy * 2 < paged_sm_count() / 2) a.per_cta >>= 1;
   a.head_groups = hy;
   const long ctas = (a.rows + a.per_cta - 1) / a.per_cta * hy;
   if (ctas > INT32_MAX) { set_error("paged append: %ld rows of %d heads", a.rows, a.pool.H); return KVD_ERR_ARG; }
