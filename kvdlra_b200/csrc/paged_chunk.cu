@@ -48,8 +48,8 @@ namespace kvd {
 constexpr int kPcRows = 256, kPcTok = 128;  // rows of a unit, tokens of a tile
 constexpr int kPcSub = 64;                  // tokens of a subtile: S has two buffers of them
 constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, issuer, planner (and 2 that wait)
-// registers per thread of the five warpgroups: a softmax thread holds its row
-// of S, a loader its share of a tile's codes; their sum is what the CTA is
+// registers per thread of the five warpgroups: a softmax thread holds a subtile's
+// row of S, a loader its share of a tile's codes; their sum is what the CTA is
 // launched with (96 a thread)
 constexpr int kPcRegsLaunch = 65536 / kPcThreads / 8 * 8;
 constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
