@@ -9,10 +9,15 @@
 //                      f16 and written to shared memory as rows of 64 dims with
 //                      the 128-byte swizzle: the same image is a K-major operand
 //                      of the scores and an MN-major one of the values.
-//   issuer (1 warp)    S_w = Q_w K^T for the two row tiles w of 128 rows, and
-//                      O_w += P_w V with P_w in TMEM, by subtiles of 64 tokens.
-//                      S has two buffers per row tile: the next scores are there
-//                      while this subtile's weights are computed.
+//   issuers (a warp for each row tile w of 128 rows)  S_w = Q_w K^T, and O_w +=
+//                      P_w V with P_w in TMEM, by subtiles of 64 tokens.  S has two
+//                      buffers per row tile: the next scores are there while this
+//                      subtile's weights are computed.  P lies over S's columns, so
+//                      the next scores wait for the product that reads it: products
+//                      of different accumulators are in no order otherwise.  One
+//                      issuer for both row tiles, waiting for each in turn, took
+//                      1.40 ms where two take 1.26 (below), but 196 us against 220
+//                      for 96 requests of 32 rows (head_dim 128).
 //   softmax (2 x 4 warps)  a thread owns a row (a TMEM lane): the row's maxima
 //                      and sums need no other thread.  S is read once, in one wait
 //                      (TMEM reads are slow beside the tensor core); P_w (f16) goes
@@ -32,7 +37,7 @@
 //
 // Bound, per tile of 256 rows x 128 tokens at head_dim 128, in clocks: tensor
 // core 2048, exponentials 2176 (8 a warp), shared memory 2500 (Q and K once per
-// subtile, V, the converted tiles).  Measured: 4900, 1.3 ms and 818 TFLOP/s for
+// subtile, V, the converted tiles).  Measured: 4700, 1.26 ms and 847 TFLOP/s for
 // 2048 queries of 32768 tokens with 32 heads over 8 (int8 pages, bf16).  S of 128
 // tokens in one buffer (fewer reads of Q, the softmax waits for it) took as long;
 // the exponentials' share, or the count of the softmax's instructions, made no
@@ -47,14 +52,14 @@ namespace kvd {
 
 constexpr int kPcRows = 256, kPcTok = 128;  // rows of a unit, tokens of a tile
 constexpr int kPcSub = 64;                  // tokens of a subtile: S has two buffers of them
-constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, issuer, planner (and 2 that wait)
+constexpr int kPcThreads = 640;            // 8 softmax warps, 8 loaders, 2 issuers, planner (and 1 that waits)
 // registers per thread of the five warpgroups: a softmax thread holds a subtile's
 // row of S, a loader its share of a tile's codes; their sum is what the CTA is
 // launched with (96 a thread)
 constexpr int kPcRegsLaunch = 65536 / kPcThreads / 8 * 8;
 constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
-constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544;
+constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544, kPcIssue1 = 576;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
 constexpr long kPcPolls = 1L << 20;
 
@@ -135,7 +140,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   __shared__ ChunkScales scales[L::ring];
   __shared__ uint64_t kf[NS], ke[NS], vf[NS], ve[NS];  // a stage of keys, of values: full, empty
   __shared__ uint64_t sf[2][2], pf[2][2];              // scores, weights of (row tile, S buffer)
-  __shared__ uint64_t of[2], od[2], qf[2], drain;      // a subtile's product into O, a unit's last one; queries
+  __shared__ uint64_t of[2], od[2], qf[2], drain[2];   // a subtile's product into O, a unit's last one; queries
   __shared__ uint64_t nf[kPcPieces], ne[kPcPieces];    // pieces
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) {
@@ -146,9 +151,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
     dead = 0;
     for (int i = 0; i < NS; ++i) {
       umma::mbar_init(kf + i, 128);
-      umma::mbar_init(ke + i, 1);
+      umma::mbar_init(ke + i, 2);
       umma::mbar_init(vf + i, 128);
-      umma::mbar_init(ve + i, 1);
+      umma::mbar_init(ve + i, 2);
     }
     for (int w = 0; w < 2; ++w) {
       for (int b = 0; b < 2; ++b) {
@@ -158,12 +163,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
       umma::mbar_init(of + w, 1);
       umma::mbar_init(od + w, 1);
       umma::mbar_init(qf + w, 128);
+      umma::mbar_init(drain + w, 1);
     }
     for (int i = 0; i < kPcPieces; ++i) {
       umma::mbar_init(nf + i, 1);
-      umma::mbar_init(ne + i, 256 + 256 + 1);
+      umma::mbar_init(ne + i, 256 + 256 + 2);
     }
-    umma::mbar_init(&drain, 1);
     umma::mbar_fence_init();
   }
   umma::fence_before_sync();
@@ -202,17 +207,20 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         if (!more) break;
       }
       a.part.head[blockIdx.x] = begun;
-    } else if (warp == kPcIssue0 / 32) {
-      // ----------------------------------------------------------- issuer
-      // the whole warp walks, one lane issues: descriptors stay in uniform registers
+    } else if (warp == kPcIssue0 / 32 || warp == kPcIssue1 / 32) {
+      // ---------------------------------------------------------- issuers
+      // The whole warp walks, one lane issues: descriptors stay in uniform registers.
+      // A row tile that has no rows takes no part (its softmax threads may be units
+      // ahead); its issuer then gives the stages back and nothing else.
+      const int w = warp == kPcIssue0 / 32 ? 0 : 1;
       const uint64_t k_d = umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::k), 16, 1024);
       const uint32_t hi = (uint32_t)(k_d >> 32), k_lo = (uint32_t)k_d;
-      const uint32_t q_lo = k_lo - ((L::k - L::q) >> 4);  // an address counts 16 bytes
+      const uint32_t q_w = k_lo - ((L::k - L::q) >> 4) + w * (L::tile >> 4);  // an address counts 16 bytes
       const uint32_t v_lo = (uint32_t)umma::smem_desc_sw128((uint32_t)__cvta_generic_to_shared(psm + L::v), kPcBlock, 1024);
       constexpr uint32_t id_s = umma::idesc_f16(128, kPcSub, false), id_o = umma::idesc_f16(128, D, true);
       // subtile b of a stage, S buffer b
-      auto scores = [&](int w, int stage, int b) {
-        const uint32_t q_w = q_lo + w * (L::tile >> 4), k_s = k_lo + stage * (L::tile >> 4) + b * (kPcSub * 128 >> 4);
+      auto scores = [&](int stage, int b) {
+        const uint32_t k_s = k_lo + stage * (L::tile >> 4) + b * (kPcSub * 128 >> 4);
         if (umma::elect_one()) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         }
         __syncwarp();
       };
-      auto values = [&](int w, int stage, int b, bool acc) {
+      auto values = [&](int stage, int b, bool acc) {
         const uint32_t v_s = v_lo + stage * (L::tile >> 4) + b * (kPcSub * 128 >> 4);
         if (umma::elect_one()) {
 #pragma unroll
@@ -238,64 +246,68 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
         __syncwarp();
       };
       auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
-      int it = 0, t0 = 0, t1 = 0, un1 = 0;  // tiles so far, of all units and by row tile; units of the second
+      int it = 0, t = 0, uq = 0;  // tiles of all units and of this row tile's, units of it
       bool ok = true;
       for (int un = 0;; ++un) {
         const int sl = un % kPcPieces;
         ok = wait_all(nf + sl, (un / kPcPieces) & 1);
         if (!ok) break;
         const int n = __shfl_sync(0xffffffffu, pieces[sl].n, 0);
-        const bool two = __shfl_sync(0xffffffffu, pieces[sl].rows - pieces[sl].row0 > 128, 0);
+        const bool active = __shfl_sync(0xffffffffu, w == 0 || pieces[sl].rows - pieces[sl].row0 > 128, 0);
         if (lane == 0) umma::mbar_arrive(ne + sl);
         if (n == 0) break;
-        // a row tile that has no rows takes no part: its threads may be units ahead
-        ok = wait_all(qf, un & 1) && (!two || wait_all(qf + 1, un1++ & 1)) && wait_all(kf + it % NS, (it / NS) & 1);
+        if (!active) {
+          for (int i = 0; i < n && ok; ++i) {
+            const int g = it + i, st = g % NS;
+            ok = wait_all(kf + st, (g / NS) & 1) && wait_all(vf + st, (g / NS) & 1);
+            if (ok && lane == 0) {
+              umma::mbar_arrive(ke + st);
+              umma::mbar_arrive(ve + st);
+            }
+          }
+          if (!ok) break;
+          it += n;
+          continue;
+        }
+        ok = wait_all(qf + w, uq++ & 1) && wait_all(kf + it % NS, (it / NS) & 1);
         if (!ok) break;
         umma::fence_after_sync();
-        for (int b = 0; b < 2; ++b) {
-          scores(0, it % NS, b);
-          if (two) scores(1, it % NS, b);
-        }
+        scores(it % NS, 0);
+        scores(it % NS, 1);
         commit(ke + it % NS);
         for (int i = 0; i < n && ok; ++i) {
           const int g = it + i, st = g % NS, nx = (g + 1) % NS;
           const bool more = i + 1 < n;
           ok = wait_all(vf + st, (g / NS) & 1);
           for (int b = 0; b < 2 && ok; ++b) {
-            // O += P V of this subtile, then S of the next tile's over its P: the
-            // tensor core takes one thread's products in order
-            ok = wait_all(&pf[0][b], t0 & 1);
+            // O += P V of this subtile, then S of the next tile's over its P.  The two
+            // have accumulators of their own, so nothing but the wait for the first
+            // keeps the second from P's columns while they are read.
+            ok = wait_all(&pf[w][b], t & 1);
             if (!ok) break;
             umma::fence_after_sync();
-            values(0, st, b, i > 0 || b > 0);
+            values(st, b, i > 0 || b > 0);
             if (b == 0 && more) {
               ok = wait_all(kf + nx, ((g + 1) / NS) & 1);
               if (!ok) break;
-              umma::fence_after_sync();
             }
-            if (more) scores(0, nx, b);
-            if (two) {
-              ok = wait_all(&pf[1][b], t1 & 1);
-              if (!ok) break;
-              umma::fence_after_sync();
-              values(1, st, b, i > 0 || b > 0);
-              if (more) scores(1, nx, b);
-            }
+            ok = wait_all(of + w, b);  // two products a tile: the parity is the subtile's
+            if (!ok) break;
+            umma::fence_after_sync();
+            if (more) scores(nx, b);
           }
           if (!ok) break;
-          ++t0;
-          if (two) ++t1;
+          ++t;
           commit(ve + st);
           if (more) commit(ke + nx);
         }
         if (!ok) break;
-        commit(od);
-        if (two) commit(od + 1);
+        commit(od + w);
         it += n;
       }
       if (!ok) {  // nothing may be in flight when TMEM is freed
-        commit(&drain);
-        umma::mbar_wait_bounded(&drain, 0, kPcPolls);
+        commit(drain + w);
+        umma::mbar_wait_bounded(drain + w, 0, kPcPolls);
       }
     }
   } else if (warp >= kPcLoad0 / 32) {
