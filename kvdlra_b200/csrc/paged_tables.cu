@@ -283,8 +283,8 @@ extern "C" int kvd_page_tables(int32_t batch, int32_t max_pages, int32_t page_si
   // launch, which spreads them over the SMs, makes it 7.3, 7.7 and 7.8.
   const bool one = (long)capacity + batch <= 8192;
   const void* scan = one ? (const void*)kvd::paged_tables_kernel<true> : (const void*)kvd::paged_tables_kernel<false>;
-  if (smem > 48 * 1024)
-    if (int rc = ensure_smem(scan, smem, "paged_tables_kernel")) return rc;
+  // always: the default limit counts the kernel's static memory too
+  if (int rc = ensure_smem(scan, smem, "paged_tables_kernel")) return rc;
   if (one) {
     KTimerScope kts_("paged_tables_kernel", s);
     kvd::paged_tables_kernel<true><<<1, kvd::kTabThreads, smem, s>>>(a);
