@@ -217,10 +217,13 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
       const int np = ((t_seg1 + page_mask) >> lg) - pg0;
       __syncthreads();  // the previous segment's (or unit's) readers are done
       for (int i = tid; i < np; i += kRowThreads) {
-        int id = a.table[(long)b * a.table_stride + pg0 + i];
-        if (id < 0 || id >= pool.num_pages) {
-          pool.flag(kStatusBounds, kPagedBadPage);
-          id = -1;
+        int id = -1;  // of a page that no row of the piece sees: the tile begins before the window, or in the padding
+        if (pg0 + i >= lo >> lg && ((pg0 + i) << lg) < hi) {
+          id = a.table[(long)b * a.table_stride + pg0 + i];
+          if (id < 0 || id >= pool.num_pages) {
+            pool.flag(kStatusBounds, kPagedBadPage);
+            id = -1;
+          }
         }
         const float vs = id < 0 ? 0.f : pool.vs[(long)id * pool.scale_stride + h];
         seg[i] = make_float4(id < 0 ? 0.f : pool.ks[(long)id * pool.scale_stride + h], vs, log2f(vs), __int_as_float(id));

@@ -40,3 +40,22 @@ assert ok and want == [t.tolist(), p.lens.tolist(), p.cu_new.tolist(), p.slots.t
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("n", [1, 40])  # the few-row kernel, the tensor-memory kernel
+@pytest.mark.parametrize("page", [16, 64])
+def test_pages_that_nobody_sees_need_no_id(n, page) -> None:
+    """A server gives the pages behind the window back; padding needs none."""
+    case = _Case("e4m3", 64, 2, page, [300, 301], seed=31)
+    q = torch.randn(2, 8, n, 64, device=DEV).to(torch.bfloat16)
+    want = paged_attention(case.pool, case.table, case.lens, q, window=20)
+    t = case.table.clone()
+    t[:, : (300 - n + 1 - 20) // page] = -1
+    assert torch.equal(paged_attention(case.pool, t, case.lens, q, window=20), want)
+    case.pool.check_status()
+    starts = _i32([0, 200])
+    want = paged_attention(case.pool, case.table, case.lens, q, starts=starts)
+    t = case.table.clone()
+    t[1, : 200 // page] = 1 << 30
+    assert torch.equal(paged_attention(case.pool, t, case.lens, q, starts=starts), want)
+    case.pool.check_status()
