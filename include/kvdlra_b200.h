@@ -327,8 +327,9 @@ int kvd_paged_append(const kvd_paged_pool* pool, const int32_t* slots, int32_t b
                      kvd_hf_view k, kvd_hf_view v, kvd_stream_t stream);
 
 /* Dense keys and values of the first out_k.tokens tokens of each request, in
- * the model dtype (the return value a model's own attention reads); rows from
- * lens[b] on are zero.  batch <= 32767. */
+ * the model dtype (the return value a model's own attention reads), held to its
+ * range (a code may round up past the largest value); rows from lens[b] on are
+ * zero.  batch <= 32767. */
 int kvd_paged_peek(const kvd_paged_pool* pool, int32_t batch, const int32_t* table, int64_t table_stride,
                    int32_t max_pages, const int32_t* lens, int32_t dtype, kvd_hf_view out_k,
                    kvd_hf_view out_v, kvd_stream_t stream);

@@ -6,6 +6,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -35,6 +36,15 @@ template <> struct IO<__half> {
   static KVD_DEVICE float load(const __half* p) { return __half2float(*p); }
   static KVD_DEVICE void store(__half* p, float v) { *p = __float2half_rn(v); }
 };
+
+// Values read back, and averages of them, held to their type's range: a code may
+// round up past it (65504 in f16 is 256 x 256 in e4m3).  NaN stays.
+template <typename T> KVD_DEVICE float finite_max() {
+  return sizeof(T) == 4 ? 3.402823466e38f : std::is_same<T, __half>::value ? 65504.f : 3.389531390e38f;
+}
+template <typename T> KVD_DEVICE void store_held(T* p, float v) {
+  store_f(p, fabsf(v) > finite_max<T>() ? copysignf(finite_max<T>(), v) : v);
+}
 
 // Four codes (the bytes of w) as two f16 pairs, exactly: both formats have at
 // most 8 significant bits and stay within f16's normal and subnormal range.
@@ -406,7 +416,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPar
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int k = 0; k < V; ++k) store_f(dst + 32 * V * c + k, o[c][k] * f);
+      for (int k = 0; k < V; ++k) store_held(dst + 32 * V * c + k, o[c][k] * f);
     if (lane == 0 && out.lse) out.lse[row * out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
   }
 }

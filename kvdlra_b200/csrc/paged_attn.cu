@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
       if (whole_unit) {
         const long row = pc.out_row(R);
         const int hq = h * rq.G + R % rq.G;
-        store_f(reinterpret_cast<T*>(a.out.out) + (row * a.out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
+        store_held(reinterpret_cast<T*>(a.out.out) + (row * a.out.Hq + hq) * D + d, L == 0.f ? 0.f : o / L);
         if (d == 0 && a.out.lse)
           a.out.lse[row * a.out.Hq + hq] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
       } else {

@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
               uint4 v;
               T* t = reinterpret_cast<T*>(&v);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) store_f(t + k, __uint_as_float(o[e + k]) * f);
+              for (int k = 0; k < 8; ++k) store_held(t + k, __uint_as_float(o[e + k]) * f);
               *reinterpret_cast<uint4*>(dst + 32 * c + e) = v;
             }
           } else {

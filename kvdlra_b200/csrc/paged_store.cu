@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
 // -------------------------------------------------------------------- peek
 //
 // Dense keys and values of requests, (B, H, T, D) in the model's type: row t
-// is code * scale, zero from the request's length on.  One 16-byte store per
+// is code * scale, held to the type's range, zero from the request's length on.  One 16-byte store per
 // thread and step, neighbouring threads on neighbouring bytes.  HBM bounds it:
 // one byte read and 2 or 4 written per value (four prompts of 8191 tokens, 8 heads
 // of 128, to f16: 32 us, 6.3 TB/s).
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256) paged_peek_kernel(const __grid_constant__
       float f[4];
       codes_to_f32<STORE>(w[i][q], f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) store_f(v + 4 * q + k, f[k] * sc[i]);
+      for (int k = 0; k < 4; ++k) store_held(v + 4 * q + k, f[k] * sc[i]);
     }
     *reinterpret_cast<uint4*>(out + (long)t * a.st[kv] + c) = r;
   }

@@ -292,7 +292,8 @@ def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor) -> None:
 
 def paged_peek(pool: PagedPool, table: Tensor, lens: Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
     """Dense keys and values ``(B, H, tokens, D)`` of each request's first
-    ``tokens`` tokens; zero from its length on."""
+    ``tokens`` tokens, held to ``dtype``'s range (a code may round up past its
+    largest value); zero from its length on."""
     code = _DTYPES.get(dtype)
     if code is None:
         raise NotImplementedError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
@@ -324,7 +325,8 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     request, if known; it only chooses kernels.  ``scaling`` is positive, ``D ** -0.5``
     if not given.  Lengths beyond the table's columns end with them; ``cu_q``
     entries that are no offsets into the rows answer nothing.  The pages' codes are
-    finite, as :func:`paged_append` writes them.
+    finite, as :func:`paged_append` writes them.  Sums are fp32: scores and values up to
+    2^90 stay within it; the output is held to its type's range.
 
     Returns ``(B, T, Hq, D)``, or ``(rows, Hq, D)`` packed, in ``q``'s type
     (rows behind ``cu_q[B]`` are zero, or as they were in ``out``), and with

@@ -59,3 +59,59 @@ def test_pages_that_nobody_sees_need_no_id(n, page) -> None:
     t[1, : 200 // page] = 1 << 30
     assert torch.equal(paged_attention(case.pool, t, case.lens, q, starts=starts), want)
     case.pool.check_status()
+
+
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [32, 128])
+def test_the_largest_values_come_back_finite(store, dtype, dim) -> None:
+    """A code may round up past the type's largest value; the value read back is held to that."""
+    top = torch.finfo(dtype).max
+    pool = _pool(store, 2, 1, 16, dim)
+    x = torch.zeros(16, 1, dim, dtype=dtype, device=DEV)
+    x[0, 0, 0], x[1, 0, 1], x[2, 0, 2] = top, -top, top * 0.97
+    paged_append(pool, _i32(list(range(16))), x, x)
+    k, v = paged_peek(pool, _i32([[0]]), _i32([16]), 16, dtype=dtype)
+    want = _exact_peek(pool, store).clip(-top, top)
+    for y in (k, v):
+        assert np.array_equal(y[0, 0].double().cpu().numpy(), torch.tensor(want).to(dtype).double().numpy())
+    assert k[0, 0, 0, 0].item() == top and k[0, 0, 1, 1].item() == -top
+    pool.check_status()
+
+
+def _exact_peek(pool, store):
+    return pool.k[0, 0].float().double().cpu().numpy() * pool.k_scale[0, 0].double().item()
+
+
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_over_the_largest_f16_values_is_finite(store, dim, n) -> None:
+    """65504 is stored as 65536 (code 256 or 64): an average of such values is above
+    65520 less 2^-11 of it at the most, so every output rounds to 65504 or would to infinity."""
+    pool = _pool(store, 4, 1, 16, dim)
+    k = torch.randn(40, 1, dim, device=DEV).half()
+    v = torch.full((40, 1, dim), 65504.0, device=DEV).half()
+    v[:, :, 1::2] *= -1
+    paged_append(pool, _i32(list(range(40))), k, v)
+    q = torch.randn(1, 4, n, dim, device=DEV).half()
+    out = paged_attention(pool, _i32([[0, 1, 2]]), _i32([40]), q)
+    assert bool((out[..., ::2] == 65504).all()) and bool((out[..., 1::2] == -65504).all())
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, torch.bfloat16), (128, torch.float32)])
+@pytest.mark.parametrize("n", [1, 30])
+@pytest.mark.parametrize("tokens", [70, 5000])
+def test_values_up_to_2_to_the_90(dim, dtype, n, tokens) -> None:
+    rng = np.random.default_rng(4)
+    pool = _pool("e4m3", tokens // 64 + 1, 1, 64, dim)
+    k, v = (torch.tensor(rng.standard_normal((tokens, 1, dim)), dtype=torch.float32, device=DEV) for _ in "kv")
+    v = (v * 2.0**90 / v.abs().max()).contiguous()
+    paged_append(pool, torch.arange(tokens, dtype=torch.int32, device=DEV), k, v)
+    table, lens = torch.arange(tokens // 64 + 1, dtype=torch.int32, device=DEV)[None], _i32([tokens])
+    dk, dv = (x[0].double().cpu().numpy() for x in paged_peek(pool, table, lens, tokens, dtype=torch.float32))
+    q = torch.tensor(rng.standard_normal((1, 2, n, dim)), dtype=dtype, device=DEV)
+    out = paged_attention(pool, table, lens, q)
+    vs = np.repeat(pool.v_scale[:, 0].double().cpu().numpy(), 64)[None, :tokens]
+    ref, le, *parts = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), dk, dv, dim**-0.5, vs=vs)
+    assert (np.abs(out[0].double().cpu().numpy() - ref) <= P.bounds(ref, le, *parts, dim, tokens, dtype)[0]).all()
