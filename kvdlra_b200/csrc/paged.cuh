@@ -116,11 +116,8 @@ struct PagedReqs {
   int min_rows, max_rows;  // requests with rows in [min_rows, max_rows] belong to this launch
   KVD_DEVICE int q0(int b) const { return cu_q ? cu_q[b] : 0; }
   // query tokens of request b, whatever cu_q holds: within [0, q_tokens]
-  KVD_DEVICE int q_len(int b) const {
-    if (!cu_q) return q_tokens;
-    const int lo = cu_q[b], hi = cu_q[b + 1];
-    return lo < 0 || hi > q_tokens || hi < lo ? 0 : hi - lo;
-  }
+  KVD_DEVICE int q_len(int b) const { return !cu_q ? q_tokens : in_rows(b) ? cu_q[b + 1] - cu_q[b] : 0; }
+  KVD_DEVICE bool in_rows(int b) const { return cu_q[b] >= 0 && cu_q[b + 1] <= q_tokens && cu_q[b + 1] >= cu_q[b]; }
   KVD_DEVICE int len(int b) const { return max(0, min(lens[b], max_len)); }
   KVD_DEVICE int start(int b) const { return starts ? max(0, starts[b]) : 0; }
   KVD_DEVICE bool mine(int q) const { return (long)q * G >= min_rows && (long)q * G <= max_rows; }
@@ -322,13 +319,26 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(PagedReqs rq, PagedPar
   __shared__ float sums[4][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 u = part.head[blockIdx.x];
-  if (fill_tail && rq.cu_q) {  // rows behind the last request: zeros
-    const long from = (long)max(0, min(rq.cu_q[rq.batch], rq.q_tokens)) * out.Hq, to = (long)rq.q_tokens * out.Hq;
-    const long stride = (long)gridDim.x * gridDim.y * 128;
-    const long at = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 128 + threadIdx.x;
-    for (long e = from * D + at; e < to * D; e += stride) store_f(reinterpret_cast<T*>(out.out) + e, 0.f);
-    if (out.lse)
-      for (long e = from + at; e < to; e += stride) out.lse[e] = -INFINITY;
+  if (fill_tail && rq.cu_q) {  // rows that no request answers: zeros
+    bool odd = false;            // offsets that are none into the rows
+    for (int b = threadIdx.x; b < rq.batch; b += 128) odd |= !rq.in_rows(b);
+    odd = __syncthreads_or(odd);
+    const long ctas = (long)gridDim.x * gridDim.y, cta = (long)blockIdx.y * gridDim.x + blockIdx.x;
+    auto clear = [&](long from, long to, long at, long stride) {  // rows [from, to)
+      for (long e = from * out.Hq * D + at; e < to * out.Hq * D; e += stride) store_f(reinterpret_cast<T*>(out.out) + e, 0.f);
+      if (out.lse)
+        for (long e = from * out.Hq + at; e < to * out.Hq; e += stride) out.lse[e] = -INFINITY;
+    };
+    if (!odd) {
+      clear(0, rq.cu_q[0], cta * 128 + threadIdx.x, ctas * 128);
+      clear(rq.cu_q[rq.batch], rq.q_tokens, cta * 128 + threadIdx.x, ctas * 128);
+    } else {
+      for (long r = cta; r < rq.q_tokens; r += ctas) {
+        bool answered = false;
+        for (int b = threadIdx.x; b < rq.batch; b += 128) answered |= rq.in_rows(b) && r >= rq.cu_q[b] && r < rq.cu_q[b + 1];
+        if (!__syncthreads_or(answered)) clear(r, r + 1, threadIdx.x, 128);
+      }
+    }
   }
   if (u.w == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -329,7 +329,7 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     2^90 stay within it; the output is held to its type's range.
 
     Returns ``(B, T, Hq, D)``, or ``(rows, Hq, D)`` packed, in ``q``'s type
-    (rows behind ``cu_q[B]`` are zero, or as they were in ``out``), and with
+    (rows that no request answers are zero, or as they were in ``out``), and with
     ``return_lse`` the natural log of the softmax's sum, fp32, without the last
     dimension (-inf where a query saw nothing)."""
     dtype = _dtype(q, "queries")
@@ -354,7 +354,7 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     _no_grad(q)
     q, view = _rows(q)
     lse = None
-    fill = out is None  # rows behind the last request
+    fill = out is None  # rows that no request answers
     if out is None:
         out = torch.empty_like(q) if packed and q.is_contiguous() else q.new_empty(shape)
     else:

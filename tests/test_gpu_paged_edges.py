@@ -115,3 +115,32 @@ def test_values_up_to_2_to_the_90(dim, dtype, n, tokens) -> None:
     vs = np.repeat(pool.v_scale[:, 0].double().cpu().numpy(), 64)[None, :tokens]
     ref, le, *parts = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), dk, dv, dim**-0.5, vs=vs)
     assert (np.abs(out[0].double().cpu().numpy() - ref) <= P.bounds(ref, le, *parts, dim, tokens, dtype)[0]).all()
+
+
+def _stale(shape, dtype):
+    """Memory of a freed tensor full of sevens, which the allocator hands out next."""
+    for _ in range(4):
+        x = torch.full(shape, 7.0, dtype=dtype, device=DEV)
+        del x
+
+
+@pytest.mark.parametrize("dtype, scale", [(torch.float32, 1), (torch.bfloat16, 1), (torch.bfloat16, 12)])
+@pytest.mark.parametrize("cu, live", [([2, 5, 5], [2, 3, 4]), ([0, 9, 5], []), ([-3, 2, 5], [2, 3, 4]), ([5, 2, 900], []), ([0, 3, 900], [0, 1, 2]),
+                                      ([1, 3, 6], [1, 2, 3, 4, 5]), ([7, 7, 7], [])])
+def test_rows_that_no_request_answers_are_zero(dtype, scale, cu, live) -> None:
+    """Rows before the first offset, behind the last, and of offsets that make no
+    sense: zeros in an output that the call makes, left alone in the caller's."""
+    case = _Case("int8", 64, 1, 16, [90, 80], seed=6)
+    rows = 7 * scale
+    cu = [c * scale for c in cu]
+    live = sorted(r for x in live for r in range(x * scale, (x + 1) * scale))
+    q = torch.randn(rows, 2, 64, device=DEV).to(dtype)
+    mine = torch.full_like(q, 5.0)
+    paged_attention(case.pool, case.table, case.lens, q, cu_q=_i32(cu), out=mine)
+    _stale(q.shape, dtype)
+    _stale(q.shape[:2], torch.float32)
+    out, lse = paged_attention(case.pool, case.table, case.lens, q, cu_q=_i32(cu), return_lse=True)
+    dead = [r for r in range(rows) if r not in live]
+    assert not out[dead].any() and bool((lse[dead] == -torch.inf).all())
+    assert bool((mine[dead] == 5.0).all())
+    assert torch.equal(mine[live], out[live]) and bool(out[live].any(-1).all()) and bool(lse[live].isfinite().all())
