@@ -618,7 +618,7 @@ extern "C" int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, co
   if (batch == 0 || q_tokens == 0) return KVD_OK;
   const int G = num_q_heads / H;
   if ((int64_t)q_tokens * G > INT32_MAX / 2 || (int64_t)max_pages * pool->page_size > INT32_MAX / 2) { set_error("paged attention: too many rows or cached tokens for one request"); return KVD_ERR_ARG; }
-  if (!table || !lens || !q || !out) { set_error("paged attention: null pointer"); return KVD_ERR_ARG; }
+  if ((!table && max_pages) || !lens || !q || !out) { set_error("paged attention: null pointer"); return KVD_ERR_ARG; }
   const int size = dtype == KVD_DTYPE_F32 ? 4 : 2;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)(q_sb * size) | (uintptr_t)(q_sh * size) | (uintptr_t)(q_st * size)) % 16) {
     set_error("paged attention: queries, their strides and the output must be multiples of 16 bytes");

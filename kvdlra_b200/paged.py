@@ -365,8 +365,8 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
         lse = q.new_empty(shape[:-1], dtype=torch.float32)
         if packed and not fill:
             lse.fill_(-torch.inf)
-    if batch == 0 or table.shape[1] == 0:  # nobody has tokens
-        if fill or not packed:
+    if batch == 0:
+        if fill:
             out.zero_()
         if lse is not None:
             lse.fill_(-torch.inf)

@@ -144,3 +144,12 @@ def test_rows_that_no_request_answers_are_zero(dtype, scale, cu, live) -> None:
     assert not out[dead].any() and bool((lse[dead] == -torch.inf).all())
     assert bool((mine[dead] == 5.0).all())
     assert torch.equal(mine[live], out[live]) and bool(out[live].any(-1).all()) and bool(lse[live].isfinite().all())
+
+
+def test_queries_over_a_table_without_columns_are_zero_in_the_callers_output() -> None:
+    pool = PagedPool.allocate(4, 16, 2, 64, device=DEV)
+    q = torch.randn(6, 4, 64, device=DEV)
+    mine = torch.full_like(q, 5.0)
+    table = torch.empty((2, 0), dtype=torch.int32, device=DEV)
+    out, lse = paged_attention(pool, table, _i32([0, 3]), q, cu_q=_i32([1, 2, 4]), out=mine, return_lse=True)
+    assert not out[1:4].any() and bool((out[[0, 4, 5]] == 5.0).all()) and bool((lse == -torch.inf).all())
