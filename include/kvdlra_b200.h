@@ -301,7 +301,8 @@ typedef struct kvd_paged_pool {
  * table entries, lens[b] = cached + new (may be cached_lens), *free_left (may
  * be free_count), cu_new [batch + 1] (exclusive prefix sums of new_lens), and
  * per row of the step its slot (page * page_size + offset) and its position;
- * rows [cu_new[batch], capacity) get slot -1 and position 0.  When pages, table
+ * rows [cu_new[batch], capacity) get slot -1 and position 0; rows of a page whose
+ * id is negative or too large for a slot get slot -1 and set the status bit.  When pages, table
  * columns or rows do not suffice, or a length is negative, nothing is
  * allocated: every slot is -1, cu_new 0, lens = cached_lens, and the status
  * bit is set.  batch <= 12288. */

@@ -6,7 +6,8 @@
 // its j-th new page is free[count - 1 - (P_b + j)] (the free list is a stack);
 // row i of the step belongs to the request with cu_b <= i < cu_{b+1}, cu the
 // exclusive prefix sum of t, at position p = c_b + i - cu_b and slot
-// table[b][p / S] * S + p % S.  Rows behind the last request get slot -1.
+// table[b][p / S] * S + p % S.  Rows behind the last request get slot -1, and so do,
+// with a status bit, rows of a page whose id in the table names none.
 //
 // A few integers per request and row: latency bounds it, the writes of slots and
 // positions where there are a million rows.  A small step is one launch of one
@@ -14,6 +15,7 @@
 // rows and the table's new entries; a row's page is looked up in the table or on
 // the stack, whichever holds it, so the grid's CTAs need nothing of one another.
 #include <algorithm>
+#include <climits>
 
 #include "paged.cuh"
 
@@ -80,8 +82,12 @@ KVD_DEVICE void table_rows(const TableArgs& a, const int* cu, const int* pp, F c
           page_no = pn;
           const int have = (c + mask) >> a.lg_page;
           id = pn < have ? a.table[(long)b * a.table_stride + pn] : a.free_pages[top - 1 - (pp[b] + pn - have)];
+          if (id < 0 || id > INT_MAX >> a.lg_page) {  // names no page: its tokens go nowhere
+            id = -1;
+            if (a.status) atomicOr(a.status + kStatusBounds, kPagedBadPage);
+          }
         }
-        s[i] = (id << a.lg_page) + (q[i] & mask);
+        s[i] = id < 0 ? -1 : (id << a.lg_page) + (q[i] & mask);
       }
     }
     if (wide && r0 + 4 <= a.capacity) {

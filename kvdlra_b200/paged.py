@@ -198,7 +198,8 @@ def build_page_tables(cached_lens: Tensor, new_lens: Tensor, table: Tensor, free
     rows of slots and positions are written.  ``in_place``: the new lengths and
     the free count overwrite ``cached_lens`` and ``free_count``.  If pages,
     columns or rows do not suffice, or a length is negative, nothing is
-    allocated, every slot is -1, and ``status`` (int32, 4 words) says so."""
+    allocated, every slot is -1, and ``status`` (int32, 4 words) says so; it says so
+    too of a token whose page has no id in ``table``, which gets slot -1."""
     device = cached_lens.device
     batch = cached_lens.shape[0]
     _ints(cached_lens, (batch,), "cached_lens", device)

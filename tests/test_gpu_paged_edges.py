@@ -153,3 +153,23 @@ def test_queries_over_a_table_without_columns_are_zero_in_the_callers_output() -
     table = torch.empty((2, 0), dtype=torch.int32, device=DEV)
     out, lse = paged_attention(pool, table, _i32([0, 3]), q, cu_q=_i32([1, 2, 4]), out=mine, return_lse=True)
     assert not out[1:4].any() and bool((out[[0, 4, 5]] == 5.0).all()) and bool((lse == -torch.inf).all())
+
+
+@pytest.mark.parametrize("rows", [2, 9000])  # one launch, two launches
+@pytest.mark.parametrize("bad", [-1, -(1 << 20), 1 << 28])
+def test_ids_that_name_no_page_are_reported_by_the_tables(rows, bad) -> None:
+    """The page that a new token continues has no id, or one whose slots pass 32
+    bits: the token goes nowhere, and the status says so."""
+    pages = -(-rows // 16) + 1
+    status = torch.zeros(4, dtype=torch.int32, device=DEV)
+    table = torch.full((2, pages + 1), -1, dtype=torch.int32, device=DEV)
+    table[0, 0], table[1, 0] = 3, bad
+    p = build_page_tables(_i32([5, 3]), _i32([1, rows]), table, torch.arange(9, 9 + pages, dtype=torch.int32, device=DEV), _i32([pages]),
+                          page_size=16, capacity=rows + 1, status=status)
+    slots = p.slots.tolist()
+    assert slots[0] == 3 * 16 + 5
+    n = min(rows, 13)
+    assert slots[1 : 1 + n] == [-1] * n
+    assert all(s >= 9 * 16 for s in slots[1 + n :])
+    assert status[1].item() != 0
+    assert p.positions.tolist()[:3] == [5, 3, 4]
