@@ -39,6 +39,7 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128, 256)
 _STORES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _NAMES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_INT_MAX = 2**31 - 1  # the C calls' sizes; ctypes would cut larger ones
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -77,7 +78,7 @@ def _ints(t: Tensor, shape: tuple[int, ...], what: str, device: torch.device) ->
 
 
 def _table(t: Tensor, batch: int | None, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or (batch is not None and t.shape[0] != batch):
+    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or t.shape[1] > _INT_MAX or (batch is not None and t.shape[0] != batch):
         raise ValueError(f"table must be int32 (batch{'' if batch is None else ' ' + str(batch)}, pages) with contiguous rows, got "
                          f"{t.dtype} {tuple(t.shape)}")
     if t.device != device:
@@ -210,7 +211,7 @@ def build_page_tables(cached_lens: Tensor, new_lens: Tensor, table: Tensor, free
     if status is not None:
         _ints(status, (4,), "status", device)
     _need(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}, got {page_size}")
-    _need(capacity >= 0, f"capacity must be >= 0, got {capacity}")
+    _need(0 <= capacity <= _INT_MAX, f"capacity must be >= 0 and within 32 bits, got {capacity}")
     _cuda(device)
     # one allocation: slots and positions first, both on 16-byte borders
     cap = (capacity + 3) & ~3
@@ -375,6 +376,7 @@ def paged_attention(pool: PagedPool, table: Tensor, lens: Tensor, q: Tensor, *, 
     ws = torch.empty(pool.workspace_bytes(dtype, hq), dtype=torch.uint8, device=device)
     _call(device, N.lib().kvd_paged_attention, "kvd_paged_attention", pool._ref, batch, table.data_ptr(), table.stride(0), table.shape[1],
           lens.data_ptr(), None if starts is None else starts.data_ptr(), None if cu_q is None else cu_q.data_ptr(), dtype,
-          view.ptr, view.stride_b, view.stride_h, view.stride_t, tokens, max_q, hq, dim**-0.5 if scaling is None else scaling, window,
+          view.ptr, view.stride_b, view.stride_h, view.stride_t, tokens, min(max_q, _INT_MAX), hq,
+          dim**-0.5 if scaling is None else scaling, min(window, _INT_MAX),
           out.data_ptr(), None if lse is None else lse.data_ptr(), int(fill), ws.data_ptr(), ws.numel(), _stream(device.index))
     return out if lse is None else (out, lse)

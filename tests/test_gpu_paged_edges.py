@@ -173,3 +173,11 @@ def test_ids_that_name_no_page_are_reported_by_the_tables(rows, bad) -> None:
     assert all(s >= 9 * 16 for s in slots[1 + n :])
     assert status[1].item() != 0
     assert p.positions.tolist()[:3] == [5, 3, 4]
+
+
+def test_sizes_past_32_bits_are_not_cut() -> None:
+    case = _Case("int8", 64, 1, 16, [60, 50], seed=8)
+    q = torch.randn(2, 2, 1, 64, device=DEV)
+    want = paged_attention(case.pool, case.table, case.lens, q)
+    assert torch.equal(paged_attention(case.pool, case.table, case.lens, q, window=2**32 + 5), want)
+    assert torch.equal(paged_attention(case.pool, case.table, case.lens, q[:, :, 0], cu_q=_i32([0, 1, 2]), max_q=2**32 + 1), want[:, 0])

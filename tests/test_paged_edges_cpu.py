@@ -1,0 +1,17 @@
+"""Calls of the 8-bit paged cache at the edges of what its documentation allows,
+as far as the host sees them."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kvdlra_b200.paged import build_page_tables
+
+
+@pytest.mark.parametrize("capacity", [2**31, 2**32 + 5])
+def test_capacities_past_32_bits_are_refused(capacity) -> None:
+    z = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="capacity"):
+        build_page_tables(z, z, torch.zeros(3, 4, dtype=torch.int32), torch.arange(9, dtype=torch.int32), torch.ones(1, dtype=torch.int32),
+                          page_size=16, capacity=capacity)
