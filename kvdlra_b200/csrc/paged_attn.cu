@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_per_sm(D, NT, sizeof(T) == 4
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       int e = (int)(__float_as_uint(amax) >> 23) - 127;
-      e = e > 127 ? 0 : max(-100, min(100, e));  // an infinite row keeps its values
+      e = e > 127 ? 0 : max(-100, min(126, e));  // an infinite row keeps its values
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int kk = 0; kk < KW; ++kk) {

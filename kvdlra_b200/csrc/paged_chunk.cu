@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
           for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(load_f(e + k)));
         }
         int e2 = (int)(__float_as_uint(amax) >> 23) - 127;
-        e2 = e2 > 127 ? 0 : max(-100, min(100, e2));  // an infinite row keeps its values
+        e2 = e2 > 127 ? 0 : max(-100, min(126, e2));  // an infinite row keeps its values
         const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
         cq = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scaling;
         unsigned char* dst = psm + L::q + w * L::tile + (r >> 3) * 1024 + (r & 7) * 128;

@@ -181,3 +181,26 @@ def test_sizes_past_32_bits_are_not_cut() -> None:
     want = paged_attention(case.pool, case.table, case.lens, q)
     assert torch.equal(paged_attention(case.pool, case.table, case.lens, q, window=2**32 + 5), want)
     assert torch.equal(paged_attention(case.pool, case.table, case.lens, q[:, :, 0], cu_q=_i32([0, 1, 2]), max_q=2**32 + 1), want[:, 0])
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 30])
+def test_queries_near_the_top_of_their_type(dim, dtype, n) -> None:
+    """Queries of 2^120 over keys of 2^-100: scores of ordinary size."""
+    pool = _pool("e4m3", 6, 1, 16, dim)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    k = torch.randn(70, 1, dim, device=DEV, generator=g) * 2.0**-97
+    v = torch.randn(70, 1, dim, device=DEV, generator=g)
+    paged_append(pool, _i32(list(range(70))), k, v)
+    table, lens = _i32([[0, 1, 2, 3, 4]]), _i32([70])
+    dk, dv = (x[0].double().cpu().numpy() for x in paged_peek(pool, table, lens, 70, dtype=torch.float32))
+    q = (torch.randn(1, 2, n, dim, device=DEV, generator=g) * 2.0**120).to(dtype)
+    assert bool(q.isfinite().all())
+    scaling = 2.0**-23 * dim**-0.5
+    out, lse = paged_attention(pool, table, lens, q, scaling=scaling, return_lse=True)
+    vs = np.repeat(pool.v_scale[:5, 0].double().cpu().numpy(), 16)[None, :70]
+    ref, le, *parts = P.attention(q[0].transpose(0, 1).double().cpu().numpy(), dk, dv, scaling, vs=vs)
+    tol, tol_e = P.bounds(ref, le, *parts, dim, 70, dtype)
+    assert (np.abs(out[0].double().cpu().numpy() - ref) <= tol).all()
+    assert (np.abs(lse[0].double().cpu().numpy() - le) <= tol_e).all()
