@@ -570,15 +570,16 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
               umma::tmem_wait_st();
             }
           }
-          // ---- weights: p vs 2^(m - mv) = 2^(x - m + d), d = log2(vs) + m - mv, d >= -100
-          // (a smaller scale's values are nothing beside the row's largest); their sum
-          // over a page's tokens, times 2^-d, goes to l
+          // ---- weights: p vs 2^(m - mv) = 2^(x - m + d), d = log2(vs) + m - mv; their sum
+          // over a page's tokens, times 2^-d, goes to l.  d ends at -40: x - m is 14 at
+          // most, so P is 2^-26 or less there, 0 in f16, while l's share keeps weights
+          // down to 2^-86
           const float base = m == -INFINITY ? 0.f : -m;
           const float dm = mv == -INFINITY ? 0.f : m - mv;
           uint32_t p16[32];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const float d = fmaxf(lv[g] + dm, -100.f), bg = base + d;
+            const float d = fmaxf(lv[g] + dm, -40.f), bg = base + d;
             const uint64_t c2 = pack2(cg[g], cg[g]), b2 = pack2(bg, bg);
             uint64_t l2 = pack2(0.f, 0.f);
 #pragma unroll

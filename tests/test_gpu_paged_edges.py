@@ -204,3 +204,24 @@ def test_queries_near_the_top_of_their_type(dim, dtype, n) -> None:
     tol, tol_e = P.bounds(ref, le, *parts, dim, 70, dtype)
     assert (np.abs(out[0].double().cpu().numpy() - ref) <= tol).all()
     assert (np.abs(lse[0].double().cpu().numpy() - le) <= tol_e).all()
+
+
+def test_small_weights_of_pages_without_values_count() -> None:
+    """One token ahead of 65535 others by 26.15 powers of two, whose values are all
+    zero (scale 2^-100): their weights are 8.8e-4 of the sum.  152 requests over the
+    same pages, so that a request is one CTA's.  The sum of 65536 terms, 16 at a time
+    into one of fp32, is off by 4112 half steps of 2^-24 at most, 2.5e-4."""
+    n, page = 65536, 128
+    pool = PagedPool.allocate(n // page, page, 1, 64, storage="int8", device=DEV)
+    k, v = torch.zeros(2, n, 1, 64, device=DEV).to(torch.bfloat16)
+    k[0, 0, 0], v[0] = 1.0, 30000.0
+    paged_append(pool, torch.arange(n, dtype=torch.int32, device=DEV), k, v)
+    assert pool.v_scale[1, 0].item() == 2.0**-100
+    q = torch.zeros(152, 32, 1, 64, device=DEV).to(torch.bfloat16)
+    q[..., 0] = 145.0
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV).repeat(152, 1)
+    _, lse = paged_attention(pool, table, torch.full((152,), n, dtype=torch.int32, device=DEV), q, return_lse=True)
+    ks = pool.k_scale[0, 0].item()
+    s0 = 145.0 * 0.125 * float(pool.k[0, 0, 0, 0].item()) * ks
+    want = s0 + np.log1p((n - 1) * np.exp(-s0))
+    assert float((lse.double() - want).abs().max()) <= 2.6e-4
