@@ -320,8 +320,9 @@ int kvd_page_release(int32_t batch, int32_t max_pages, int32_t page_size, const 
 
 /* Store keys and values (batch, H, tokens, D): row b * tokens + t goes to
  * slots[b * tokens + t]; a negative slot is skipped.  Rows that go to one page
- * must follow one another with ascending slots (as kvd_page_tables gives
- * them), and a page's slots fill from its first one on.  A page's scale is the
+ * must follow one another with consecutive slots, one run a call (as
+ * kvd_page_tables gives them; rows that go back into the page of the row before
+ * are skipped and set the status bit), and a page's slots fill from its first one on.  A page's scale is the
  * least power of two that fits its largest value; it grows with later calls,
  * and the codes before them are then rounded again. */
 int kvd_paged_append(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,

@@ -8,8 +8,9 @@ namespace kvd {
 
 // ------------------------------------------------------------------ append
 //
-// Row i of the call goes to slots[i].  Rows that follow one another into one
-// page are a run; a run's page gets, per KV head, the scale
+// Row i of the call goes to slots[i].  Rows that follow one another into
+// consecutive slots of one page are a run, a page's only one in the call; a run's
+// page gets, per KV head, the scale
 //   s = code_scale(max |x| over the run), if the run begins at the page's first slot
 //   s = max(that, the page's scale), otherwise; where the scale grew, the
 //       codes of the slots before the run are rounded again to the new one
@@ -90,8 +91,12 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
     }
     if (i >= a.per_cta) break;
     i0 = i + 1;
-    const int slot = slot_sm[i + 1];
+    const int slot = slot_sm[i + 1], prev = slot_sm[i];
     if (slot < 0) continue;
+    if (prev >= 0 && (prev >> lg) == (slot >> lg)) {  // its page's run has ended: it would race with this one
+      if (tid == 0) pool.flag(kStatusBounds, kPagedBadSlot);
+      continue;
+    }
     int n = 1;
     while (i + n < span) {
       const int k = i + n;

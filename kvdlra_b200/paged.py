@@ -270,8 +270,9 @@ class PageTables:
 def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor) -> None:
     """Store keys and values ``(B, H, T, D)``, or packed ``(T, H, D)``, at
     ``slots`` (int32, one per row, batch-major).  Negative slots are skipped.
-    Rows of one page must follow one another with ascending slots, as
-    :func:`build_page_tables` gives them.
+    Rows of one page must follow one another with consecutive slots, one run a call,
+    as :func:`build_page_tables` gives them; rows that go back into the page of the row
+    before (the same slot twice, a gap) are skipped and reported.
 
     A page's scale is the least power of two with ``|x| <= 448 s`` (e4m3) or
     ``127 s`` (int8); when later tokens need a larger one, the page's codes are

@@ -14,7 +14,7 @@ import pytest
 import torch
 
 import paged_plain as P
-from test_gpu_paged import DEV, _Case, _i32, _pool
+from test_gpu_paged import DEV, _Case, _data, _i32, _pool
 
 from kvdlra_b200.paged import PagedPool, build_page_tables, paged_append, paged_attention, paged_peek
 
@@ -225,3 +225,30 @@ def test_small_weights_of_pages_without_values_count() -> None:
     s0 = 145.0 * 0.125 * float(pool.k[0, 0, 0, 0].item()) * ks
     want = s0 + np.log1p((n - 1) * np.exp(-s0))
     assert float((lse.double() - want).abs().max()) <= 2.6e-4
+
+
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("page, dim", [(16, 32), (128, 128)])
+@pytest.mark.parametrize("slots, kept", [
+    ([5, 5], [5, -1]), ([3, 5], [3, -1]), ([6, 4], [6, -1]), ([0, 0, 1, 2], [0, -1, -1, -1]), ([4, 5, 7, 8, 20], [4, 5, -1, -1, -1]),
+    ([3, 4, 3, 5], [3, 4, -1, -1]), ([7, 8, 8, 9], [7, 8, -1, -1]),
+])
+def test_rows_of_a_page_out_of_order_are_skipped_and_reported(store, page, dim, slots, kept) -> None:
+    """A second run into the page that the row before went to (the same slot twice,
+    a gap, a step back) would race with the first; the rows that follow another
+    page's are stored, whatever the order of the pages."""
+    rng = np.random.default_rng(7)
+    slots, kept = [page + s for s in slots], [s if s < 0 else page + s for s in kept]
+    if page == 16 and slots[-1] == 16 + 20:
+        kept[-1] = slots[-1]  # the next page: continues there
+    slots, kept = slots + [2, 3], kept + [2, 3]
+    pool = _pool(store, 6, 3, page, dim)
+    x = _data(rng, (len(slots), 3, dim), torch.bfloat16)
+    before = pool.k.float().double().cpu().numpy(), pool.k_scale.double().cpu().numpy()
+    paged_append(pool, _i32(slots), x, x)
+    want = P.append(*before, kept, x.double().cpu().numpy(), store)
+    for name in "kv":
+        assert np.array_equal(getattr(pool, name).float().double().cpu().numpy(), want[0], equal_nan=True)
+        assert np.array_equal(getattr(pool, name + "_scale").double().cpu().numpy(), want[1])
+    with pytest.raises(RuntimeError, match="bad indices"):
+        pool.check_status()
