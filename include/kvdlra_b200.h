@@ -327,6 +327,10 @@ int kvd_page_release(int32_t batch, int32_t max_pages, int32_t page_size, const 
  * and the codes before them are then rounded again. */
 int kvd_paged_append(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,
                      kvd_hf_view k, kvd_hf_view v, kvd_stream_t stream);
+/* The same with max_new, the most rows of one request (0: not known): it only
+ * chooses the launch.  kvd_paged_append takes k.tokens for it where batch > 1. */
+int kvd_paged_append_runs(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,
+                          kvd_hf_view k, kvd_hf_view v, int32_t max_new, kvd_stream_t stream);
 
 /* Dense keys and values of the first out_k.tokens tokens of each request, in
  * the model dtype (the return value a model's own attention reads), held to its

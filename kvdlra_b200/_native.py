@@ -162,6 +162,7 @@ def lib() -> C.CDLL:
     L.kvd_page_tables_workspace_bytes.restype = sz
     L.kvd_page_release.argtypes = [i32, i32, i32, vp, vp, vp, i64, vp, i32, vp, vp, vp]
     L.kvd_paged_append.argtypes = [P(PagedPool), vp, i32, i32, HFView, HFView, vp]
+    L.kvd_paged_append_runs.argtypes = [P(PagedPool), vp, i32, i32, HFView, HFView, i32, vp]
     L.kvd_paged_peek.argtypes = [P(PagedPool), i32, vp, i64, i32, vp, i32, HFView, HFView, vp]
     L.kvd_paged_attention.argtypes = [P(PagedPool), i32, vp, i64, i32, vp, vp, vp, i32, vp, i64, i64, i64, i32, i32,
                                       i32, f32, i32, vp, vp, i32, vp, sz, vp]
@@ -172,7 +173,7 @@ def lib() -> C.CDLL:
                  "kvd_factored_decode", "kvd_factored_chunk_attention", "kvd_factored_decode_heads",
                  "kvd_factored_chunk_attention_heads", "kvd_bug_step", "kvd_surprise",
                  "kvd_select_topk",
-                 "kvd_page_tables", "kvd_page_release", "kvd_paged_append", "kvd_paged_peek", "kvd_paged_attention",
+                 "kvd_page_tables", "kvd_page_release", "kvd_paged_append", "kvd_paged_append_runs", "kvd_paged_peek", "kvd_paged_attention",
                  "kvd_paged_check_status", "kvd_profile", "kvd_profile_read", "kvd_blocked_project", "kvd_rope_table"):
         getattr(L, name).restype = C.c_int
     _lib = L

@@ -32,6 +32,7 @@ struct AppendArgs {
   const void* x[2];    // keys, values
   long sb[2], sh[2], st[2];  // strides of batch, head, token (elements)
   int per_cta;         // consecutive rows whose runs one CTA takes
+  int most;            // rows of the longest run; 0: not known
   int head_groups;     // CTAs that share the heads
 };
 
@@ -291,11 +292,16 @@ static int launch_append(AppendArgs& a, cudaStream_t s) {
   const int W = std::max(1, page * D / 2048);
   const int groups = W < 4 ? 4 / W : 1;
   const int hy = (a.pool.H + groups - 1) / groups;
-  // A page's worth of rows per CTA, fewer while the grid would leave most SMs
-  // idle: single tokens are runs of their own and are taken one after another (32
-  // of them, 8 heads of 64: 3.5 us at one per CTA, 28 at sixteen); a chunk of 512
-  // rows is better left whole (4.9 us; 6.0 at four rows per CTA).
+  // A page's worth of rows per CTA where runs are long: a CTA in which no run
+  // begins is only a start (four prompts of 8191 tokens, pages of 128, 8 heads of
+  // 128: 95 us; 151 at 16 rows per CTA).  Short runs are taken one after another, so
+  // about two of the longest a CTA: 512 single tokens, the same pages: 74 us, 141 at
+  // 64 rows; pages of 64: 36 and 121; pages of 16, 8 heads of 64: 12.6 and 28 at 16.
+  // 512 runs of 5 (16 rows a CTA): 80 us, 117 at 64, 98 at two.  Fewer while the grid
+  // would leave most SMs idle: 32 single tokens of 8 heads of 64 take 3.5 us at one row
+  // per CTA, 5.1 at two, 28 at sixteen.
   a.per_cta = page;
+  while (a.most > 0 && a.per_cta > 1 && a.per_cta / 2 >= 2L * a.most) a.per_cta >>= 1;
   while (a.per_cta > 1 && (a.rows + a.per_cta - 1) / a.per_cta * hy * 2 < paged_sm_count() / 2) a.per_cta >>= 1;
   a.head_groups = hy;
   const long ctas = (a.rows + a.per_cta - 1) / a.per_cta * hy;
@@ -355,15 +361,21 @@ struct DoPeek {
 using namespace kvd_host;
 
 extern "C" int kvd_paged_append(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,
-                                kvd_hf_view k, kvd_hf_view v, kvd_stream_t stream) try {
+                                kvd_hf_view k, kvd_hf_view v, kvd_stream_t stream) {
+  return kvd_paged_append_runs(pool, slots, batch, dtype, k, v, batch > 1 ? std::max(0, k.tokens) : 0, stream);
+}
+
+extern "C" int kvd_paged_append_runs(const kvd_paged_pool* pool, const int32_t* slots, int32_t batch, int32_t dtype,
+                                     kvd_hf_view k, kvd_hf_view v, int32_t max_new, kvd_stream_t stream) try {
   kvd::AppendArgs a;
   if (int rc = paged_pool_view(pool, &a.pool)) return rc;
-  if (batch < 0 || k.tokens < 0 || k.tokens != v.tokens) { set_error("paged append: keys of %d tokens, values of %d, batch %d", k.tokens, v.tokens, batch); return KVD_ERR_ARG; }
+  if (batch < 0 || max_new < 0 || k.tokens < 0 || k.tokens != v.tokens) { set_error("paged append: keys of %d tokens, values of %d, batch %d", k.tokens, v.tokens, batch); return KVD_ERR_ARG; }
   if (batch == 0 || k.tokens == 0) return KVD_OK;
   const int size = dtype == KVD_DTYPE_F32 ? 4 : 2;
   if (!slots || !view_ok(k, size) || !view_ok(v, size)) { set_error("paged append: keys, values and their strides must be multiples of 16 bytes"); return KVD_ERR_ARG; }
   a.slots = slots;
   a.tokens = k.tokens;
+  a.most = max_new;
   a.rows = (long)batch * k.tokens;
   if (a.rows > INT32_MAX) { set_error("paged append: %ld rows", a.rows); return KVD_ERR_ARG; }
   a.x[0] = k.ptr; a.sb[0] = k.stride_b; a.sh[0] = k.stride_h; a.st[0] = k.stride_t;

@@ -11,7 +11,7 @@ A serving step is four calls, all on the current stream, with lengths, tables
 and slots on the device throughout::
 
     plan = tables.advance(new_lens, capacity)            # pages, slots, positions
-    paged_append(pool, plan.slots, k, v)                 # per layer
+    paged_append(pool, plan.slots, k, v)                 # per layer; max_new= the most new tokens of a request
     out = paged_attention(pool, tables.table, tables.lens, q, cu_q=plan.cu_new, scaling=s)
     tables.release(done)                                 # finished requests
 
@@ -267,12 +267,13 @@ class PageTables:
         _call(self.device, N.lib().kvd_paged_check_status, "kvd_paged_check_status", self.status.data_ptr(), _stream(self.device.index))
 
 
-def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor) -> None:
+def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor, *, max_new: int = 0) -> None:
     """Store keys and values ``(B, H, T, D)``, or packed ``(T, H, D)``, at
     ``slots`` (int32, one per row, batch-major).  Negative slots are skipped.
     Rows of one page must follow one another with consecutive slots, one run a call,
     as :func:`build_page_tables` gives them; rows that go back into the page of the row
-    before (the same slot twice, a gap) are skipped and reported.
+    before (the same slot twice, a gap) are skipped and reported.  ``max_new``: the most
+    rows of one packed request, if known; it only chooses the launch.
 
     A page's scale is the least power of two with ``|x| <= 448 s`` (e4m3) or
     ``127 s`` (int8); when later tokens need a larger one, the page's codes are
@@ -286,10 +287,12 @@ def paged_append(pool: PagedPool, slots: Tensor, k: Tensor, v: Tensor) -> None:
     _need(heads == pool.num_heads and k.shape[-1] == pool.head_dim, f"pool holds {pool.num_heads} heads x {pool.head_dim}, got {tuple(k.shape)}")
     _need(k.device == pool.device and v.device == pool.device, f"k and v must be on {pool.device}")
     _ints(slots, (batch * tokens,), "slots", pool.device)
+    _need(max_new >= 0, f"max_new must be >= 0, got {max_new}")
     _no_grad(k, v)
+    most = min(max_new, _INT_MAX) if k.dim() == 3 else tokens
     k, k_view = _rows(k)  # the copies, if any, live until the call is made: the allocator orders their reuse by stream
     v, v_view = _rows(v)
-    _call(pool.device, N.lib().kvd_paged_append, "kvd_paged_append", pool._ref, slots.data_ptr(), batch, dtype, k_view, v_view,
+    _call(pool.device, N.lib().kvd_paged_append_runs, "kvd_paged_append", pool._ref, slots.data_ptr(), batch, dtype, k_view, v_view, most,
           _stream(pool.device.index))
 
 

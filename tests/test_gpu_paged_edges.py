@@ -252,3 +252,38 @@ def test_rows_of_a_page_out_of_order_are_skipped_and_reported(store, page, dim, 
         assert np.array_equal(getattr(pool, name + "_scale").double().cpu().numpy(), want[1])
     with pytest.raises(RuntimeError, match="bad indices"):
         pool.check_status()
+
+
+@pytest.mark.parametrize("page, dim, heads", [(16, 64, 8), (128, 128, 3), (32, 256, 1)])
+@pytest.mark.parametrize("batch, new", [(300, 1), (70, 5), (3, 200)])
+def test_append_of_many_requests_whatever_the_launch(page, dim, heads, batch, new) -> None:
+    """Many runs a CTA or one, with and without the length of the longest run, and
+    with a wrong one: the same codes and scales."""
+    rng = np.random.default_rng(batch + page)
+    lens = [page * int(rng.integers(0, 3)) + int(rng.integers(0, page)) for _ in range(batch)]
+    held = [-(-(n + new) // page) for n in lens]
+    ids = rng.permutation(sum(held)).tolist()
+    slots, at = [], 0
+    for n, h in zip(lens, held):
+        mine, at = ids[at : at + h], at + h
+        slots += [mine[t // page] * page + t % page for t in range(n, n + new)]
+    x = [_data(rng, (batch * new, heads, dim), torch.bfloat16) for _ in "kv"]
+    pools = []
+    for kw in ({}, {"max_new": new}, {"max_new": 1}, {"max_new": 2**40}, None):
+        pool = _pool("e4m3", sum(held), heads, page, dim)
+        if kw is None:
+            paged_append(pool, _i32(slots), *(t.view(batch, new, heads, dim).transpose(1, 2) for t in x))
+        else:
+            paged_append(pool, _i32(slots), *x, **kw)
+        pool.check_status()
+        pools.append(pool)
+    n = min(batch * new, 400)  # the plain form of the first rows, whole runs
+    n -= n % new
+    before = _pool("e4m3", sum(held), heads, page, dim)
+    want = P.append(before.k.float().double().cpu().numpy(), before.k_scale.double().cpu().numpy(), slots[:n], x[0][:n].double().cpu().numpy(), "e4m3")
+    rows = sorted({s // page for s in slots[:n]})
+    assert np.array_equal(pools[0].k[rows].float().double().cpu().numpy(), want[0][rows], equal_nan=True)
+    assert np.array_equal(pools[0].k_scale[rows].double().cpu().numpy(), want[1][rows])
+    for p in pools[1:]:
+        assert torch.equal(p.k.view(torch.uint8), pools[0].k.view(torch.uint8)) and torch.equal(p.v.view(torch.uint8), pools[0].v.view(torch.uint8))
+        assert torch.equal(p.k_scale, pools[0].k_scale) and torch.equal(p.v_scale, pools[0].v_scale)
