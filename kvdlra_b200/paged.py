@@ -18,7 +18,7 @@ and slots on the device throughout::
 Every call but ``check_status`` can be captured in a CUDA graph.  Bad slots
 and page ids are skipped on the device and reported by ``check_status``.
 Inference only: there is no gradient through the codes, and inputs that
-require one are refused while gradients are recorded.  The reference has no
+require one are refused while gradients are recorded, inputs with a tangent always.  The reference has no
 counterpart of these operators.
 """
 
@@ -29,6 +29,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as N
 
@@ -93,6 +94,8 @@ def _cuda(device: torch.device) -> None:
 def _no_grad(a: Tensor, b: Tensor | None = None) -> None:
     if (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("the 8-bit paged cache is inference only: call it under torch.no_grad()")
+    if unpack_dual(a).tangent is not None or (b is not None and unpack_dual(b).tangent is not None):
+        raise NotImplementedError("the 8-bit paged cache is inference only: it carries no tangents")
 
 
 def _rows(t: Tensor) -> tuple[Tensor, N.HFView]:

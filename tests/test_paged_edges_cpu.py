@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kvdlra_b200 import paged
 from kvdlra_b200.paged import build_page_tables
 
 
@@ -15,3 +16,19 @@ def test_capacities_past_32_bits_are_refused(capacity) -> None:
     with pytest.raises(ValueError, match="capacity"):
         build_page_tables(z, z, torch.zeros(3, 4, dtype=torch.int32), torch.arange(9, dtype=torch.int32), torch.ones(1, dtype=torch.int32),
                           page_size=16, capacity=capacity)
+
+
+def test_tangents_are_refused() -> None:
+    """Forward-mode differentiation would end at the codes without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.ones(2, 3)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones(2, 3))
+        for args in ((d,), (x, d), (d, x)):
+            with pytest.raises(NotImplementedError, match="inference only"):
+                paged._no_grad(*args)
+        paged._no_grad(x, x)
+    paged._no_grad(x)
+    with pytest.raises(NotImplementedError, match="inference only"):
+        paged._no_grad(x, torch.ones(2, requires_grad=True))
