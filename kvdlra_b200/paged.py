@@ -215,6 +215,8 @@ def build_page_tables(cached_lens: Tensor, new_lens: Tensor, table: Tensor, free
         _ints(status, (4,), "status", device)
     _need(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}, got {page_size}")
     _need(0 <= capacity <= _INT_MAX, f"capacity must be >= 0 and within 32 bits, got {capacity}")
+    _need(not (in_place and batch and new_lens.data_ptr() == cached_lens.data_ptr()),
+          "new_lens must have memory of their own: the lengths are overwritten in place")
     _cuda(device)
     # one allocation: slots and positions first, both on 16-byte borders
     cap = (capacity + 3) & ~3

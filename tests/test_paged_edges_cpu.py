@@ -32,3 +32,13 @@ def test_tangents_are_refused() -> None:
     paged._no_grad(x)
     with pytest.raises(NotImplementedError, match="inference only"):
         paged._no_grad(x, torch.ones(2, requires_grad=True))
+
+
+def test_new_lengths_of_their_own() -> None:
+    """In place, the lengths are overwritten while the new ones are still read."""
+    z, table = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4, dtype=torch.int32)
+    free, count = torch.arange(9, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="new_lens must have memory of their own"):
+        build_page_tables(z, z, table, free, count, page_size=16, capacity=4, in_place=True)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        build_page_tables(z, z, table, free, count, page_size=16, capacity=4)
