@@ -25,7 +25,8 @@ dense peek still hold.
 
 A :class:`kvdlra_b200.PagedKVCache` tags every step, prompts included, and its
 queries are answered from the 8-bit pages (``kvd_paged_attention``: causal, the
-layer's sliding window, the cache's left padding).
+layer's sliding window, the cache's left padding).  A mask that says anything
+else is refused.
 
 An attention module carrying ``kvd_heads = (h0, hc)`` (set by
 :func:`kvdlra_b200.sharding.shard_attention_heads`) answers only the query
@@ -66,9 +67,10 @@ def factored_attention_forward(module: torch.nn.Module, query: torch.Tensor, key
     if dropout:
         raise NotImplementedError("factored attention has no dropout (inference only)")
     if hasattr(layer, "paged_attention"):
-        layer.check_mask(attention_mask, query)
-        window = kwargs.get("sliding_window") or getattr(module, "sliding_window", None) or 0
-        return layer.paged_attention(query, scaling=scaling, heads=heads, window=int(window)), None
+        window = int(kwargs.get("sliding_window") or getattr(module, "sliding_window", None) or 0)
+        causal = kwargs.get("is_causal")
+        layer.check_mask(attention_mask, query, window=window, causal=getattr(module, "is_causal", True) if causal is None else causal)
+        return layer.paged_attention(query, scaling=scaling, heads=heads, window=window), None
     mode = getattr(layer, "_mode", None)
     if mode in ("ingest", "score"):
         # a chunk (or a frozen-scoring window: its own K/V are the tail)

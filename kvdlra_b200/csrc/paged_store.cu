@@ -419,7 +419,7 @@ extern "C" int kvd_paged_check_status(int32_t* status, kvd_stream_t stream) {
   if (e != cudaSuccess) { set_error("status read: %s", cudaGetErrorString(e)); return KVD_ERR_CUDA; }
   if (h[kvd::kStatusTimeout]) { set_error("paged cache: a device wait timed out (code %d)", h[kvd::kStatusTimeout]); return KVD_ERR_TIMEOUT; }
   if (h[kvd::kStatusBounds]) {
-    set_error("paged cache: bad indices were skipped (flags %d: 1 slot, 2 page id, 4 the step's tables could not be built)", h[kvd::kStatusBounds]);
+    set_error("paged cache: bad indices were skipped (flags %d: 1 slot, 2 page id, 4 the step's tables could not be built, 8 a captured step's attention mask)", h[kvd::kStatusBounds]);
     return KVD_ERR_ARG;
   }
   if (h[kvd::kStatusNumeric]) { set_error("paged cache: values that are not finite were stored (infinities saturated, NaN as 0)"); return KVD_ERR_NUMERIC; }

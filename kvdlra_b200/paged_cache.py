@@ -27,6 +27,8 @@ from .paged import PAGE_SIZES, PagedPool, PagePlan, PageTables, paged_append, pa
 
 __all__ = ["PagedKVCache", "PagedKVLayer"]
 
+_MARK = "_kvdlra_checked"
+
 
 class PagedKVLayer(CacheLayerMixin):  # type: ignore[misc]
     """One layer's pages."""
@@ -82,17 +84,28 @@ class PagedKVLayer(CacheLayerMixin):  # type: ignore[misc]
         assert isinstance(out, Tensor)
         return out
 
-    def check_mask(self, mask: Tensor | None, query: Tensor) -> None:
-        """Refuse a padded batch that the cache was not told of.  A mask is only
-        read (which synchronises) by the first layer, at a prompt's first step."""
+    def check_mask(self, mask: Tensor | None, query: Tensor, *, window: int = 0, causal: bool = True) -> None:
+        """Refuse a mask that says anything but what the pages' attention computes:
+        causal over the cache's tokens, ``window``, the cache's left padding.  Reading
+        it synchronises: a step's mask is marked once it was read.  Under capture it
+        is compared on the device, and :meth:`PagedKVCache.check_status` raises."""
         owner = self._owner
-        if mask is None or owner.starts is not None or self._index or self.cumulative_length != query.shape[2]:
+        if mask is None:
+            if not causal and query.shape[2] > 1:
+                raise NotImplementedError("attention over the pages is causal")
             return
-        if torch.cuda.is_current_stream_capturing():
+        step, seen = getattr(mask, _MARK, (None, None))
+        if step is owner._step_mark and seen == window:
             return
-        seen = mask[:, :, -1, :] if mask.dtype == torch.bool else mask[:, :, -1, :] >= 0
-        if not bool(seen.all()):
-            raise ValueError("the attention mask hides tokens of the prompt: give the cache left_padding (tokens per row)")
+        fits = owner._mask_fits(mask, int(query.shape[2]), self.cumulative_length, window)
+        if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            assert self.pool is not None
+            self.pool.status[1:2].bitwise_or_((~fits).to(torch.int32) * 8)
+        elif not bool(fits):
+            owner._refused = True
+            raise ValueError("the attention mask is not the causal one of the cache's tokens: hidden tokens at the front of a row are "
+                             "the cache's left_padding (tokens per row), others are not supported; reset() the cache")
+        setattr(mask, _MARK, (owner._step_mark, window))
 
     def get_mask_sizes(self, query_length: int) -> tuple[int, int]:
         if isinstance(query_length, Tensor):  # tolerate cache_position tensors
@@ -154,6 +167,7 @@ class PagedKVCache(Cache):
         self._plan: PagePlan | None = None
         self._at: tuple[int, int] | None = None
         self._new: dict[int, Tensor] = {}
+        self._step_mark, self._refused = object(), False
         super().__init__(layers=[PagedKVLayer(self, i) for i in range(num_layers)])
 
     def _reads_pages(self) -> bool:
@@ -176,6 +190,8 @@ class PagedKVCache(Cache):
         assert tables is not None
         if batch != tables.batch:
             raise NotImplementedError(f"PagedKVCache was initialised for batch size {tables.batch}, got {batch}")
+        if self._refused:
+            raise RuntimeError("a step of this cache was refused half way: reset() it")
         if self._at != (length, tokens):
             if self._at is not None and length != sum(self._at):
                 raise RuntimeError(f"a layer holds {length} tokens, the cache {sum(self._at)}: its layers advance together")
@@ -185,8 +201,28 @@ class PagedKVCache(Cache):
                 self._new[tokens] = torch.full((batch,), tokens, dtype=torch.int32, device=tables.device)
             self._plan = tables.advance(self._new[tokens], batch * tokens)
             self._at = (length, tokens)
+            self._step_mark = object()
         assert self._plan is not None
         return self._plan
+
+    def _mask_fits(self, mask: Tensor, tokens: int, length: int, window: int) -> Tensor:
+        """Whether a mask ``(1 or B, 1 or heads, tokens, length)``, of truth values or
+        to be added, is the pages' own (a truth value on its device).  Rows of padding
+        queries, which mean nothing, may say anything."""
+        if mask.dim() != 4 or tuple(mask.shape[2:]) != (tokens, length):
+            return torch.zeros((), dtype=torch.bool, device=mask.device)
+        t, last = torch.arange(length, device=mask.device), torch.arange(length - tokens, length, device=mask.device)[:, None]
+        seen = t <= last
+        if window:
+            seen &= t > last - window
+        if self.starts is not None:
+            starts = self.starts.to(mask.device)[:, None, None, None]
+            seen = seen & (t >= starts)
+        # to be added: 0, or so low that nothing is left of the token's weight
+        fits = mask == seen if mask.dtype == torch.bool else torch.where(seen, mask == 0, mask <= -1e4)
+        if self.starts is not None:
+            fits = fits | (last < starts)
+        return fits.all()
 
     @contextmanager
     def ingesting(self) -> Iterator[None]:
@@ -201,6 +237,7 @@ class PagedKVCache(Cache):
         if self.tables is not None:
             self.tables.release(torch.ones(self.tables.batch, dtype=torch.bool, device=self.tables.device))
         self._plan = self._at = None
+        self._refused = False
         for layer in self.layers:
             layer.reset()
 
