@@ -26,7 +26,7 @@ dense peek still hold.
 A :class:`kvdlra_b200.PagedKVCache` tags every step, prompts included, and its
 queries are answered from the 8-bit pages (``kvd_paged_attention``: causal, the
 layer's sliding window, the cache's left padding).  A mask that says anything
-else is refused.
+else is refused, and so are capped scores and attention sinks.
 
 An attention module carrying ``kvd_heads = (h0, hc)`` (set by
 :func:`kvdlra_b200.sharding.shard_attention_heads`) answers only the query
@@ -67,6 +67,9 @@ def factored_attention_forward(module: torch.nn.Module, query: torch.Tensor, key
     if dropout:
         raise NotImplementedError("factored attention has no dropout (inference only)")
     if hasattr(layer, "paged_attention"):
+        for name in ("softcap", "s_aux"):
+            if kwargs.get(name) is not None:
+                raise NotImplementedError(f"attention over the pages has no {name}")
         window = int(kwargs.get("sliding_window") or getattr(module, "sliding_window", None) or 0)
         causal = kwargs.get("is_causal")
         layer.check_mask(attention_mask, query, window=window, causal=getattr(module, "is_causal", True) if causal is None else causal)

@@ -10,6 +10,7 @@ import torch
 from transformers import Gemma3ForCausalLM, Gemma3TextConfig, LlamaConfig, LlamaForCausalLM, MistralConfig, MistralForCausalLM
 
 from kvdlra_b200 import PagedKVCache, enable_factored_decode, paged_cache
+from kvdlra_b200.attention import factored_attention_forward
 from kvdlra_b200.paged import PagePlan
 
 
@@ -214,3 +215,18 @@ def test_a_mask_is_read_once_a_step(monkeypatch) -> None:
         reads.clear()
         _run(_model(kind), True, [(_ids(2, 4), {}), (_ids(2, 1), {}), (_ids(2, 1), {})])
         assert not reads
+
+
+@pytest.mark.parametrize("kw, what", [(dict(softcap=30.0), "softcap"), (dict(s_aux=torch.zeros(4)), "s_aux"), (dict(dropout=0.1), "dropout")])
+def test_parts_of_attention_that_the_pages_lack_are_refused(kw, what) -> None:
+    """Models pass them as keyword arguments; None stands for their absence."""
+    model = _model("llama")
+    enable_factored_decode(model)
+    cache = PagedKVCache(model, 32)
+    module = model.model.layers[0].self_attn
+    q, k = torch.randn(2, 4, 3, 16), torch.randn(2, 2, 3, 16)
+    key, value = cache.update(k, k, 0)
+    with torch.no_grad():
+        factored_attention_forward(module, q, key, value, None, scaling=0.25, softcap=None, s_aux=None)
+        with pytest.raises(NotImplementedError, match=what):
+            factored_attention_forward(module, q, key, value, None, scaling=0.25, **kw)
