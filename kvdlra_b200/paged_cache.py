@@ -166,7 +166,6 @@ class PagedKVCache(Cache):
         self.tables: PageTables | None = None
         self._plan: PagePlan | None = None
         self._at: tuple[int, int] | None = None
-        self._new: dict[int, Tensor] = {}
         self._step_mark, self._refused = object(), False
         super().__init__(layers=[PagedKVLayer(self, i) for i in range(num_layers)])
 
@@ -197,9 +196,8 @@ class PagedKVCache(Cache):
                 raise RuntimeError(f"a layer holds {length} tokens, the cache {sum(self._at)}: its layers advance together")
             if length + tokens > self.max_tokens:
                 raise ValueError(f"{length + tokens} tokens in a cache for {self.max_tokens}")
-            if tokens not in self._new:
-                self._new[tokens] = torch.full((batch,), tokens, dtype=torch.int32, device=tables.device)
-            self._plan = tables.advance(self._new[tokens], batch * tokens)
+            new = torch.full((batch,), tokens, dtype=torch.int32, device=tables.device)  # not kept: a captured step's belongs to its graph
+            self._plan = tables.advance(new, batch * tokens)
             self._at = (length, tokens)
             self._step_mark = object()
         assert self._plan is not None

@@ -16,6 +16,7 @@ import torch
 import paged_plain as P
 from test_gpu_paged import DEV, _Case, _data, _i32, _pool
 
+from kvdlra_b200 import PagedKVCache
 from kvdlra_b200.paged import PagedPool, build_page_tables, paged_append, paged_attention, paged_peek
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +288,21 @@ def test_append_of_many_requests_whatever_the_launch(page, dim, heads, batch, ne
     for p in pools[1:]:
         assert torch.equal(p.k.view(torch.uint8), pools[0].k.view(torch.uint8)) and torch.equal(p.v.view(torch.uint8), pools[0].v.view(torch.uint8))
         assert torch.equal(p.k_scale, pools[0].k_scale) and torch.equal(p.v_scale, pools[0].v_scale)
+
+
+def test_a_cache_after_a_capture_that_never_ran() -> None:
+    """Nothing that a captured step made is used by an eager one."""
+    cache = PagedKVCache(None, 64, page_size=16, num_layers=1)
+    k = torch.randn(2, 2, 5, 64, device=DEV).to(torch.bfloat16)
+    cache.update(k, k, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.update(k[:, :, :1], k[:, :, :1], 0)
+    del graph
+    cache.reset()
+    cache.update(k, k, 0)
+    got = cache.update(k[:, :, :1], k[:, :, :1], 0)[0]
+    assert cache.tables.lens.tolist() == [6, 6]
+    assert torch.equal(got[:, :, 5], got[:, :, 0])
+    cache.check_status()
