@@ -360,6 +360,12 @@ int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, const int32_t
                         kvd_stream_t stream);
 size_t kvd_paged_attention_workspace_bytes(const kvd_paged_pool* pool, int32_t dtype, int32_t num_q_heads);
 
+/* How long a wait inside kvd_paged_attention's kernel for chunks may last before
+ * it gives up, sets the status word and returns: SM clocks, < 0: not at all, 0
+ * (the default): by the amount of work, a second at the least.  Process-wide, for
+ * tests of that path. */
+int kvd_paged_wait_limit(int64_t clocks);
+
 /* Read and clear the status words of a pool or of page tables (synchronises
  * the stream). */
 int kvd_paged_check_status(int32_t* status, kvd_stream_t stream);

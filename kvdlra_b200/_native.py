@@ -169,12 +169,13 @@ def lib() -> C.CDLL:
     L.kvd_paged_attention_workspace_bytes.argtypes = [P(PagedPool), i32, i32]
     L.kvd_paged_attention_workspace_bytes.restype = sz
     L.kvd_paged_check_status.argtypes = [vp, vp]
+    L.kvd_paged_wait_limit.argtypes = [i64]
     for name in ("kvd_check_status", "kvd_prefill", "kvd_append", "kvd_consolidate", "kvd_absorb_block", "kvd_peek",
                  "kvd_factored_decode", "kvd_factored_chunk_attention", "kvd_factored_decode_heads",
                  "kvd_factored_chunk_attention_heads", "kvd_bug_step", "kvd_surprise",
                  "kvd_select_topk",
                  "kvd_page_tables", "kvd_page_release", "kvd_paged_append", "kvd_paged_append_runs", "kvd_paged_peek", "kvd_paged_attention",
-                 "kvd_paged_check_status", "kvd_profile", "kvd_profile_read", "kvd_blocked_project", "kvd_rope_table"):
+                 "kvd_paged_check_status", "kvd_paged_wait_limit", "kvd_profile", "kvd_profile_read", "kvd_blocked_project", "kvd_rope_table"):
         getattr(L, name).restype = C.c_int
     _lib = L
     return L

@@ -43,6 +43,8 @@
 // the exponentials' share, or the count of the softmax's instructions, made no
 // difference.  Loaders of one warpgroup, and 16 softmax warps with half a row each,
 // ran out of registers.
+#include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -61,7 +63,11 @@ constexpr int kPcRegsSoftmax = 128, kPcRegsLoad = 80, kPcRegsIssue = 64;
 static_assert(2 * kPcRegsSoftmax + 2 * kPcRegsLoad + kPcRegsIssue <= 5 * kPcRegsLaunch, "register split");
 constexpr int kPcLoad0 = 256, kPcIssue0 = 512, kPcPlan0 = 544, kPcIssue1 = 576;
 constexpr int kPcBlock = kPcTok * 128;     // bytes of 64 columns of a 128-row f16 operand
-constexpr long kPcPolls = 1L << 20;
+// A wait gives up after a second's clocks and 70 us for each tile of the CTA's share
+// (which the planner and an idle row tile may have to wait for whole; a tile takes 3
+// to 4): time, counted in steps of 2^16 clocks.
+constexpr int kPcClockShift = 16, kPcWaitBase = 1 << 15, kPcWaitTile = 2;
+constexpr long kPcPolls = 1L << 20;  // of the last wait, for products that are on their way
 
 struct ChunkArgs {
   PagedPool pool;
@@ -73,6 +79,7 @@ struct ChunkArgs {
   float scaling;  // times log2(e)
   PagedOut out;
   PagedPart part;
+  int wait_limit;  // steps of the clock, < 0: none at all, 0: by the work
 };
 
 struct alignas(16) ChunkScales {  // of one tile, per 16 tokens
@@ -132,6 +139,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   unsigned char* psm = psm_raw + (-(int)(uint32_t)__cvta_generic_to_shared(psm_raw) & 1023);  // swizzle atoms are aligned
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;  // a wait gave up
+  __shared__ int wait_limit;     // steps of the clock
   __shared__ ChunkPiece pieces[kPcPieces];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be warp-uniform
@@ -173,13 +181,18 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
   }
   umma::fence_before_sync();
   const WorkAt at = find_work<kPcRows, kPcTok, kPcThreads>(rq, blockIdx.x, gridDim.x);  // has barriers
+  if (tid == 0) wait_limit = a.wait_limit ? (int)a.wait_limit : (int)min((long)INT_MAX, kPcWaitBase + kPcWaitTile * at.chunk);
+  __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = tmem_base;
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    for (long i = 0; i < kPcPolls; ++i) {
-      if (umma::mbar_try_wait(bar, parity)) return true;
-      if (dead) return false;
+    if (umma::mbar_try_wait(bar, parity)) return true;
+    const uint32_t since = (uint32_t)(clock64() >> kPcClockShift);
+    while (!dead && (int)((uint32_t)(clock64() >> kPcClockShift) - since) <= wait_limit) {
+      for (int i = 0; i < 32; ++i)
+        if (umma::mbar_try_wait(bar, parity)) return true;
     }
+    if (dead) return false;
     dead = 1;
     pool.flag(kStatusTimeout, 1);
     return false;
@@ -668,6 +681,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const __grid
 namespace kvd_host {
 using namespace kvd;
 
+static std::atomic<int> paged_wait_limit{0};
+
 bool paged_chunk_takes(int head_dim, int dtype) { return (head_dim == 64 || head_dim == 128) && dtype != KVD_DTYPE_F32; }
 
 size_t paged_chunk_ws_bytes(int head_dim) { return part_bytes(paged_sm_count(), kPcRows, head_dim); }
@@ -703,10 +718,16 @@ static int launch_chunk_d(ChunkArgs& a, int store, int fill_tail, void* ws, cuda
 int launch_paged_chunk(const PagedPool& pool, int D, int store, const PagedReqs& reqs, const int* table, long table_stride,
                        int dtype, const void* q, long q_sb, long q_sh, long q_st, float scaling_log2, const PagedOut& out,
                        int fill_tail, void* ws, cudaStream_t s) {
-  ChunkArgs a{pool, reqs, table, table_stride, q, q_sb, q_sh, q_st, scaling_log2, out, {}};
+  ChunkArgs a{pool, reqs, table, table_stride, q, q_sb, q_sh, q_st, scaling_log2, out, {}, paged_wait_limit.load()};
   if (dtype == KVD_DTYPE_BF16)
     return D == 64 ? launch_chunk_d<64, __nv_bfloat16>(a, store, fill_tail, ws, s) : launch_chunk_d<128, __nv_bfloat16>(a, store, fill_tail, ws, s);
   return D == 64 ? launch_chunk_d<64, __half>(a, store, fill_tail, ws, s) : launch_chunk_d<128, __half>(a, store, fill_tail, ws, s);
 }
 
 }  // namespace kvd_host
+
+extern "C" int kvd_paged_wait_limit(int64_t clocks) {
+  const int64_t steps = clocks >> kvd::kPcClockShift;
+  kvd_host::paged_wait_limit = clocks < 0 ? -1 : clocks == 0 ? 0 : (int)std::max<int64_t>(1, std::min<int64_t>(INT_MAX, steps));
+  return KVD_OK;
+}

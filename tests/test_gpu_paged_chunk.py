@@ -12,6 +12,7 @@ import torch
 import paged_plain as P
 from test_gpu_paged import DEV, _Case, _i32
 
+from kvdlra_b200 import _native as N
 from kvdlra_b200.paged import PagedPool, paged_append, paged_attention, paged_peek
 
 pytestmark = pytest.mark.gpu
@@ -77,4 +78,30 @@ def test_chunks_of_pages_past_32_bits() -> None:
     tol, tol_e = P.bounds(ref, le, *parts, dim, 300, torch.bfloat16)
     assert (np.abs(out[0].double().cpu().numpy() - ref) <= tol).all()
     assert (np.abs(lse[0].double().cpu().numpy() - le) <= tol_e).all()
+    pool.check_status()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_wait_that_runs_out_sets_the_status(dim) -> None:
+    """With no patience at all, some wait gives up (the planner, eight units
+    ahead, waits for one of 512 tiles): the call ends, the status says so, and the next call is right."""
+    n, page = 65536, 128
+    pool = PagedPool.allocate(n // page, page, 1, dim, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v = (torch.randn(n, 1, dim, device=DEV, generator=g).to(torch.bfloat16) for _ in "kv")
+    paged_append(pool, torch.arange(n, dtype=torch.int32, device=DEV), k, v)
+    table = torch.arange(n // page, dtype=torch.int32, device=DEV).repeat(1480, 1)
+    lens = torch.full((1480,), n, dtype=torch.int32, device=DEV)
+    q = torch.randn(1480, 32, 1, dim, device=DEV, generator=g).to(torch.bfloat16)
+    want = paged_attention(pool, table, lens, q)
+    pool.check_status()
+    L = N.lib()
+    try:
+        assert L.kvd_paged_wait_limit(-1) == 0
+        paged_attention(pool, table, lens, q)
+        with pytest.raises(RuntimeError, match="timed out"):
+            pool.check_status()
+    finally:
+        L.kvd_paged_wait_limit(0)
+    assert torch.equal(paged_attention(pool, table, lens, q), want)
     pool.check_status()
