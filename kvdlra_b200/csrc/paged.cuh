@@ -6,7 +6,6 @@
 #pragma once
 
 #include <algorithm>
-#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -39,11 +38,16 @@ template <> struct IO<__half> {
 
 // Values read back, and averages of them, held to their type's range: a code may
 // round up past it (65504 in f16 is 256 x 256 in e4m3).  NaN stays.
-template <typename T> KVD_DEVICE float finite_max() {
-  return sizeof(T) == 4 ? 3.402823466e38f : std::is_same<T, __half>::value ? 65504.f : 3.389531390e38f;
+KVD_DEVICE void store_held(float* p, float v) { *p = fabsf(v) == INFINITY ? copysignf(3.402823466e38f, v) : v; }
+KVD_DEVICE void store_held(__nv_bfloat16* p, float v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+  *reinterpret_cast<uint16_t*>(p) = r;
 }
-template <typename T> KVD_DEVICE void store_held(T* p, float v) {
-  store_f(p, fabsf(v) > finite_max<T>() ? copysignf(finite_max<T>(), v) : v);
+KVD_DEVICE void store_held(__half* p, float v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.f16.f32 %0, %1;" : "=h"(r) : "f"(v));
+  *reinterpret_cast<uint16_t*>(p) = r;
 }
 
 // Four codes (the bytes of w) as two f16 pairs, exactly: both formats have at
