@@ -541,15 +541,23 @@ int paged_pool_view(const kvd_paged_pool* p, PagedPool* out) {
 }
 
 // A request of at most this many rows goes to the few-row kernel: its codes are
-// read once per 8 or 16 rows, the tensor-memory kernel's once per 256.  At 32 rows
-// (96 requests of 4 drafted tokens, head_dim 128) the first takes 203 us, the other
-// 190.
-constexpr int kFewRows = 16;
+// read once per 8 or 16 rows, the tensor-memory kernel's once per 256, whose tile
+// costs the same however few rows it has.  The first and the other, in us:
+//   head_dim 64   96 requests of 100 to 4099 tokens, 4 KV heads: 140 and 178 at 17
+//                 rows, 164 and 189 at 32, 212 and 191 at 33, 312 and 195 at 64;
+//                 one of 32768, 8 KV heads: 36 and 52 at 17, 38 and 54 at 32, 44 and
+//                 55 at 33, 52 and 57 at 64
+//   head_dim 128  96 requests of 100 to 4099: 192 and 194 at 32 rows; 512 of 300 to
+//                 899: 319 and 353 at 17, 385 and 428 at 32, 499 and 428 at 33; one of
+//                 32768: 49 and 58 at 17, 52 and 61 at 32, 65 and 62 at 33
+constexpr int kFewRows = 32;
 
-// Rows of a unit / 8: one, or two where a request has more than eight rows
-// (head_dim 256: sixteen rows' accumulators would not fit the registers; thirty-two
-// rows at head_dim 64 fit, but took 237 us where sixteen take 211, for 24 fp32
-// requests of 1 to 257 rows).
+// Rows of a unit / 8: one, or two where a request has more than eight rows.  64
+// requests of 1 to 32768 tokens, 8 KV heads of 128, bf16: 442 us in units of 8 rows
+// and 632 in units of 16 at 8 rows, 799 and 707 at 9, 856 and 726 at 16; fp32: 569 and
+// 781, 1021 and 799, 1092 and 888 (head_dim 256: sixteen rows' accumulators would not
+// fit the registers; thirty-two rows at head_dim 64 fit, but took 237 us where sixteen
+// take 211, for 24 fp32 requests of 1 to 257 rows).
 static int rows_nt(long max_rows, int D) { return max_rows <= 8 || D == 256 ? 1 : 2; }
 // CTAs that fit an SM (the kernel's launch bounds)
 static int rows_ctas(int D, int nt, bool fp32) { return paged_sm_count() * rows_per_sm(D, nt, fp32); }

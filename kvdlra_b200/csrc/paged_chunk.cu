@@ -16,8 +16,8 @@
 //                      the next scores wait for the product that reads it: products
 //                      of different accumulators are in no order otherwise.  One
 //                      issuer for both row tiles, waiting for each in turn, took
-//                      1.40 ms where two take 1.26 (below), but 196 us against 220
-//                      for 96 requests of 32 rows (head_dim 128).
+//                      1.40 ms where two take 1.25 (below); with one row tile, 96
+//                      requests of 32 rows, head_dim 128, 196 us and 194 to 220.
 //   softmax (2 x 4 warps)  a thread owns a row (a TMEM lane): the row's maxima
 //                      and sums need no other thread.  S is read once, in one wait
 //                      (TMEM reads are slow beside the tensor core); P_w (f16) goes
@@ -37,7 +37,7 @@
 //
 // Bound, per tile of 256 rows x 128 tokens at head_dim 128, in clocks: tensor
 // core 2048, exponentials 2176 (8 a warp), shared memory 2500 (Q and K once per
-// subtile, V, the converted tiles).  Measured: 4700, 1.26 ms and 847 TFLOP/s for
+// subtile, V, the converted tiles).  Measured: 4700, 1.25 ms and 850 TFLOP/s for
 // 2048 queries of 32768 tokens with 32 heads over 8 (int8 pages, bf16).  S of 128
 // tokens in one buffer (fewer reads of Q, the softmax waits for it) took as long;
 // the exponentials' share, or the count of the softmax's instructions, made no

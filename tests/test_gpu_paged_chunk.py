@@ -1,4 +1,4 @@
-"""Requests of more query rows than the few-row kernel takes (17 and up: bf16 and
+"""Requests of more query rows than the few-row kernel takes (33 and up: bf16 and
 f16, head_dim 64 and 128), where the tensor-memory kernel's own order of work
 counts: the same bits from every call, alone and beside another, and pages that
 lie beyond 4 GiB."""
@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import paged_plain as P
-from test_gpu_paged import DEV, _Case, _i32
+from test_gpu_paged import DEV, _Case, _i32, _run
 
 from kvdlra_b200 import _native as N
 from kvdlra_b200.paged import PagedPool, paged_append, paged_attention, paged_peek
@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dim, dtype, store", [(64, torch.bfloat16, "e4m3"), (128, torch.float16, "int8"), (128, torch.bfloat16, "e4m3")])
-@pytest.mark.parametrize("tokens", [5, 40, 300])  # rows 20 (one row tile), 160 and 1200 (two, and units of one behind them)
+@pytest.mark.parametrize("tokens", [12, 40, 300])  # rows 48 (one row tile), 160 and 1200 (two, and units of one behind them)
 def test_repeated_chunks_give_the_same_bits(dim, dtype, store, tokens) -> None:
     """The next scores go where the weights lay that the product before reads: a
     product that ran late would show as other bits, or as a wrong row."""
@@ -92,7 +92,7 @@ def test_a_wait_that_runs_out_sets_the_status(dim) -> None:
     paged_append(pool, torch.arange(n, dtype=torch.int32, device=DEV), k, v)
     table = torch.arange(n // page, dtype=torch.int32, device=DEV).repeat(1480, 1)
     lens = torch.full((1480,), n, dtype=torch.int32, device=DEV)
-    q = torch.randn(1480, 32, 1, dim, device=DEV, generator=g).to(torch.bfloat16)
+    q = torch.randn(1480, 40, 1, dim, device=DEV, generator=g).to(torch.bfloat16)
     want = paged_attention(pool, table, lens, q)
     pool.check_status()
     L = N.lib()
@@ -105,3 +105,24 @@ def test_a_wait_that_runs_out_sets_the_status(dim) -> None:
         L.kvd_paged_wait_limit(0)
     assert torch.equal(paged_attention(pool, table, lens, q), want)
     pool.check_status()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_short_requests_of_one_row_tile(dim) -> None:
+    """Hundreds of units that fill half a pair of row tiles, several to a CTA, beside
+    one that fills both and a few of the other kernel's."""
+    lens = [40 + (37 * i) % 300 for i in range(150)]
+    case = _Case("e4m3", dim, 4, 32, lens, seed=12)
+    q_lens = [12 if i % 10 else 1 + i % 8 for i in range(150)]
+    q_lens[75] = 40
+    assert _run(case, q_lens, 4, torch.bfloat16) <= 1.0
+    case.pool.check_status()
+
+
+@pytest.mark.parametrize("dim, dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("group, tokens", [(16, 1), (17, 1), (32, 1), (33, 1), (8, 4), (11, 3), (64, 1), (1, 32), (1, 33), (43, 3)])
+def test_rows_at_the_border_of_the_two_kernels(dim, dtype, group, tokens) -> None:
+    case = _Case("int8", dim, 1, 16, [200, 33, 1], seed=13)
+    _run(case, [tokens] * 3, group, dtype)
+    _run(case, [tokens, 0, 1], group, dtype, window=20)
+    case.pool.check_status()

@@ -218,7 +218,7 @@ def test_small_weights_of_pages_without_values_count() -> None:
     k[0, 0, 0], v[0] = 1.0, 30000.0
     paged_append(pool, torch.arange(n, dtype=torch.int32, device=DEV), k, v)
     assert pool.v_scale[1, 0].item() == 2.0**-100
-    q = torch.zeros(152, 32, 1, 64, device=DEV).to(torch.bfloat16)
+    q = torch.zeros(152, 40, 1, 64, device=DEV).to(torch.bfloat16)
     q[..., 0] = 145.0
     table = torch.arange(n // page, dtype=torch.int32, device=DEV).repeat(152, 1)
     _, lse = paged_attention(pool, table, torch.full((152,), n, dtype=torch.int32, device=DEV), q, return_lse=True)
