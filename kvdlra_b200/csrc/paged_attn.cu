@@ -31,8 +31,10 @@
 // the running maxima only when these pass them by kLTop and kPTop: a tile costs
 // one vote instead of reductions over the lanes.
 //
-// Measured: 64 requests of 1 to 32768 tokens, 32 heads over 8 of 128, int8: 419 us,
-// 5.1 TB/s, 79 % of the copy rate; one of 131072 tokens, e4m3: 61 us, 4.4 TB/s.  The
+// Measured: 64 requests of 1 to 32768 tokens, 32 heads over 8 of 128, int8: 424 us,
+// 5.1 TB/s, 78 % of the copy rate; one of 131072 tokens, e4m3: 63 us, 4.2 TB/s; 64
+// ragged ones by form: fp32 of 128 517 us where the bytes take 319, bf16 of 64, 32 and
+// 256 241, 197 and 451 where they take 159, 80 and 319.  The
 // conversions' and the softmax's instructions bound it (half of all issue slots at
 // three warps a scheduler): a prefetch of the tile after next into L2 gained nothing.
 //

@@ -20,10 +20,12 @@ namespace kvd {
 //
 // A group of W warps takes a (run, head, keys or values) item: the run's rows
 // are read once, 16 bytes a load, and stay in registers between the maximum
-// and the codes (W = page * D / 2048 warps hold a whole page in 8 or 16
-// registers a lane).  A prompt's floor is HBM's (2 or 4 bytes read and one written
-// per value); four prompts of 8191 tokens, 8 heads of 128, take 69 us where that is
-// 31: a CTA's reads wait in turn for its slots.  Single tokens are latency, 3.5 us.
+// and the codes (W = page * D / 2048 warps hold a whole page, 8 or 16 loads of 16
+// bytes a lane: 32 or 64 registers).  A prompt's floor is HBM's (2 or 4 bytes read
+// and one written per value); four prompts of 8191 tokens, 8 heads of 128, take 60
+// us in f16 and 95 in bf16 where that is 31, 93 in fp32 where it is 51: a CTA's reads
+// wait in turn for its slots, and the 16-bit forms spill.  32 single tokens are
+// latency, 3.6 us (times of calls in a row, without the host).
 struct AppendArgs {
   PagedPool pool;
   const int* slots;
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(W < 4 ? 128 : 32 * W, (sizeof(T) == 2 ? 1024 :
 // is code * scale, held to the type's range, zero from the request's length on.  One 16-byte store per
 // thread and step, neighbouring threads on neighbouring bytes.  HBM bounds it:
 // one byte read and 2 or 4 written per value (four prompts of 8191 tokens, 8 heads
-// of 128, to f16: 32 us, 6.3 TB/s).
+// of 128, to f16: 33 us, 6.1 TB/s; to fp32: 55 us where the bytes take 51).
 struct PeekArgs {
   PagedPool pool;
   const int* table;
