@@ -351,7 +351,7 @@ int kvd_paged_peek(const kvd_paged_pool* pool, int32_t batch, const int32_t* tab
  * (rows, num_q_heads, D) contiguous, lse (rows, num_q_heads) or NULL: natural
  * log of the softmax sum.  Rows that no request answers (before cu_q[0], from
  * cu_q[batch] on, of offsets that are none into the rows) are left as they were,
- * or zero (lse -inf) with fill_tail. */
+ * or zero (lse -inf) with fill_tail; with batch 0 nothing is written. */
 int kvd_paged_attention(const kvd_paged_pool* pool, int32_t batch, const int32_t* table, int64_t table_stride,
                         int32_t max_pages, const int32_t* lens, const int32_t* starts, const int32_t* cu_q,
                         int32_t dtype, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
