@@ -255,7 +255,8 @@ class PageTables:
         self.device = self.table.device
 
     def advance(self, new_lens: Tensor, capacity: int) -> PagePlan:
-        """Room for ``new_lens[b]`` more tokens of each request (in place)."""
+        """Room for ``new_lens[b]`` more tokens of each request (in place: the plan's
+        ``lens`` and ``free_count`` are the tables' own, which later calls overwrite)."""
         return build_page_tables(self.lens, new_lens, self.table, self.free_pages, self.free_count, page_size=self.page_size,
                                  capacity=capacity, in_place=True, status=self.status)
 
